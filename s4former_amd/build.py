@@ -16,7 +16,10 @@ LIB_PATH = os.environ.get('S4F_LIB_OUT') or os.path.join(PKG_DIR, 'libs4f_hip.so
 SOURCES = ['gemm.hip', 'gemm2.hip', 'gemm5.hip', 'gemm6.hip', 'attention.hip', 'attn_bwd.hip', 'elementwise.hip', 'head.hip', 'eval.hip', 'pipeline.hip', 'layer.hip']
 HEADERS = ['common.h', os.path.join('..', '..', 'include', 's4f.h')]
 BASE_FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fvisibility=hidden', '-ffp-contract=off',
-              '-Wno-unused-result', '-Wno-unused-value']
+              '-Wno-unused-result', '-Wno-unused-value',
+              # no packed fp32 instructions (v_pk_add / mul / fma_f32, which -O3 makes from ordinary float code): some of their forms
+              # have given wrong results now and then.  The host pass warns that it does not know the feature: harmless.
+              '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 FLAGS = BASE_FLAGS + ['-mllvm', '-amdgpu-mfma-vgpr-form=1']
 FILE_FLAGS = {}      # per-file overrides
 # attn_bwd.hip: no SLP packing of the per-score fp32 work (v_pk_mul_f32 + the moves that pair its operands cost more issue
