@@ -191,10 +191,52 @@ int64_t s4f_attention_bwd_ws_bytes(int B, int N, int H);
 #define S4F_WS_ATTENTION_BWD 1
 #define S4F_WS_BN_SUMS 2
 #define S4F_WS_GEMM_SPLITK 3
+#define S4F_WS_QK_NORM 4        /* dims = {rows, Hq, Hk}: partial gain gradients of s4f_qk_norm_rope_bwd */
+#define S4F_WS_WGRAD_PACKED 5   /* dims = {dtype, M, N, rows (, M, N, rows ...)}: partial sums of s4f_wgrad_packed (0 = none) */
 int64_t s4f_workspace_bytes(int op, const int64_t* dims, int ndims);
 int s4f_attention_bwd_fused(const void* qkv, const void* ctx, const void* dctx, const float* lse, float* delta,
                             void* dqkv, const float* bias_u, const float* row_flag, float bias_w, int B, int N,
                             int H, void* ws, int64_t ws_bytes, s4f_stream stream);
+
+/* ------------------------------------------------------------------------------------------- norm of queries and keys + rotation
+ * One pass over the q and k heads of a projection: row r of x holds Hq query heads, then Hk key heads, 64 channels each, at
+ * x + r * ldx (a slice of the packed [B N, 3 H 64] tensor qualifies).  Per head and row, with the gain g of the head's kind [64]:
+ *   n = x g / sqrt(mean x^2 + eps)                            (gq and gk given; NULL: no norm, n = x)
+ *   y_i = n_i c_i - n_{i+32} s_i, y_{i+32} = n_{i+32} c_i + n_i s_i   (i < 32; cos and sin given; NULL: no rotation, y = n)
+ * cos / sin fp32 [period, 32], row r uses r % period (period = tokens per image: the images share positions; = rows: own ones).
+ * Sums and products fp32, rounded once to T.  y may be x itself (same ld).  All row starts 16-byte aligned.
+ * codes int8 [rows, (Hq + Hk) 64] and scales uint8 [rows, (Hq + Hk) 2] (both or NULL, norm only): an 8-bit checkpoint of the
+ * pre-norm x in the format of s4f_act_pack. */
+int s4f_qk_norm_rope_fwd(const void* x, int64_t ldx, void* y, int64_t ldy, const float* gq, const float* gk, const float* cos,
+                         const float* sin, int64_t period, float eps, int8_t* codes, uint8_t* scales, int64_t rows, int Hq, int Hk,
+                         int dtype, s4f_stream stream);
+/* Backward: dx (may be dy itself) from dy and the pre-norm x or, instead of x (NULL), its checkpoint; the gain gradients dgq / dgk
+ * fp32 [64] are written (accumulate = 0) or added to, summed over rows and heads in a fixed order.  Without the norm x, codes,
+ * dgq, dgk and ws are not used.  ws: s4f_workspace_bytes(S4F_WS_QK_NORM, {rows, Hq, Hk}). */
+int s4f_qk_norm_rope_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int8_t* codes, const uint8_t* scales,
+                         void* dx, int64_t lddx, const float* gq, const float* gk, const float* cos, const float* sin,
+                         int64_t period, float eps, float* dgq, float* dgk, int accumulate, void* ws, int64_t ws_bytes,
+                         int64_t rows, int Hq, int Hk, int dtype, s4f_stream stream);
+
+/* ------------------------------------------------------------------------------------------- activation checkpoints in 8 bits
+ * x T [rows, C] (row stride ldx) -> codes int8 [rows, C], scales uint8 [rows, C / 32]: groups of 32 channels share the least power
+ * of two s with round(max |x| / s) <= 127 (2^-126 .. 2^121), code = round-to-even(x / s), scale byte = exponent of s + 127; 255
+ * marks a group that holds an infinity or a NaN (restored as NaN).  |x - code s| <= max |x| / 127.5; code s is exact in bf16. */
+int s4f_act_pack(const void* x, int64_t ldx, int8_t* codes, uint8_t* scales, int64_t rows, int C, int dtype, s4f_stream stream);
+/* y T [rows, C] (row stride ldy) = code s */
+int s4f_act_unpack(const int8_t* codes, const uint8_t* scales, void* y, int64_t ldy, int64_t rows, int C, int dtype, s4f_stream stream);
+/* Weight gradients from checkpoints, up to four problems at once: out fp32 [M, N] (+)= dy^T x, dy T [rows, M] (row stride lddy),
+ * x = the restored [rows, N].  M % 8 == 0, N % 32 == 0.  Products exact, sums fp32 in a fixed order.
+ * ws: s4f_workspace_bytes(S4F_WS_WGRAD_PACKED, {dtype, M, N, rows, ... of each problem}). */
+typedef struct s4f_wgrad_packed_desc {
+  const void* dy; int64_t lddy;
+  const int8_t* codes; const uint8_t* scales;
+  float* out;
+  int64_t rows;
+  int32_t M, N;
+} s4f_wgrad_packed_desc;      /* 56 bytes */
+int s4f_wgrad_packed(const s4f_wgrad_packed_desc* descs, int count, int dtype, int accumulate, void* ws, int64_t ws_bytes,
+                     s4f_stream stream);
 
 /* ------------------------------------------------------------------------------------------- encoder layer (round 3)
  * TransformerEncoderLayer.forward (vit.py:113-127: LN -> MultiheadAttention -> +x; LN -> FFN(GELU) -> +x) and its backward as ONE

@@ -60,7 +60,23 @@ class LayerDesc(Structure):
 assert ctypes.sizeof(LayerDesc) == 568, 'LayerDesc must mirror s4f_layer_desc (include/s4f.h, static_assert in layer.hip)'
 
 
+class WgradPackedDesc(Structure):
+    """mirror of s4f_wgrad_packed_desc (include/s4f.h)"""
+    _fields_ = [('dy', c_void_p), ('lddy', c_int64), ('codes', c_void_p), ('scales', c_void_p), ('out', c_void_p), ('rows', c_int64),
+                ('M', c_int32), ('N', c_int32)]
+
+
+assert ctypes.sizeof(WgradPackedDesc) == 56, 'WgradPackedDesc must mirror s4f_wgrad_packed_desc (include/s4f.h, static_assert in wgradq8.hip)'
+
+
 _SIGS = {
+    's4f_qk_norm_rope_fwd': [c_void_p, c_int64, c_void_p, c_int64] + [c_void_p] * 4 + [c_int64, c_float, c_void_p, c_void_p, c_int64, c_int,
+                             c_int, c_int, c_void_p],
+    's4f_qk_norm_rope_bwd': [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64] + [c_void_p] * 4 +
+                            [c_int64, c_float, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p],
+    's4f_act_pack': [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p],
+    's4f_act_unpack': [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p],
+    's4f_wgrad_packed': [POINTER(WgradPackedDesc), c_int, c_int, c_int, c_void_p, c_int64, c_void_p],
     's4f_encoder_layer_fwd': [POINTER(LayerDesc), c_void_p],
     's4f_encoder_layer_bwd': [POINTER(LayerDesc), c_void_p, c_void_p, c_void_p],
     's4f_gemm': [POINTER(GemmDesc), c_void_p],

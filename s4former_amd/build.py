@@ -13,7 +13,8 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, 'csrc')
 OBJ_DIR = os.path.join(CSRC, '_obj')
 LIB_PATH = os.environ.get('S4F_LIB_OUT') or os.path.join(PKG_DIR, 'libs4f_hip.so')      # S4F_LIB_OUT: experiment builds beside the shipped one
-SOURCES = ['gemm.hip', 'gemm2.hip', 'gemm5.hip', 'gemm6.hip', 'attention.hip', 'attn_bwd.hip', 'elementwise.hip', 'head.hip', 'eval.hip', 'pipeline.hip', 'layer.hip']
+SOURCES = ['gemm.hip', 'gemm2.hip', 'gemm5.hip', 'gemm6.hip', 'attention.hip', 'attn_bwd.hip', 'elementwise.hip', 'head.hip', 'eval.hip', 'pipeline.hip', 'layer.hip',
+           'qknorm.hip', 'actq8.hip', 'wgradq8.hip']
 HEADERS = ['common.h', os.path.join('..', '..', 'include', 's4f.h')]
 BASE_FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fvisibility=hidden', '-ffp-contract=off',
               '-Wno-unused-result', '-Wno-unused-value',
@@ -37,13 +38,13 @@ if os.environ.get('S4F_G5_PROBES'):
     FILE_FLAGS['gemm5.hip'] = FILE_FLAGS.get('gemm5.hip', FLAGS) + ['-DG5_PROBES']
 if os.environ.get('S4F_EXTRA_DEFS'):  # experiment builds: extra -D switches for every source (space separated, e.g. "FB_PRE_ORDER=1")
     for _f in ('gemm.hip', 'gemm2.hip', 'gemm5.hip', 'gemm6.hip', 'attention.hip', 'attn_bwd.hip', 'elementwise.hip', 'head.hip',
-               'eval.hip', 'pipeline.hip', 'layer.hip'):
+               'eval.hip', 'pipeline.hip', 'layer.hip', 'qknorm.hip', 'actq8.hip', 'wgradq8.hip'):
         FILE_FLAGS[_f] = FILE_FLAGS.get(_f, FLAGS) + ['-D' + d for d in os.environ['S4F_EXTRA_DEFS'].split()]
 _DIAG = [v for v in ('S4F_FB_STAMPS', 'S4F_FB_ABL', 'S4F_G5_PROBES', 'S4F_G5P_AUTO', 'S4F_G5_ST_AUX', 'S4F_EXTRA_DEFS') if os.environ.get(v)]
 if _DIAG and not os.environ.get('S4F_LIB_OUT'):
     # stamp / ablation builds compute wrong results by construction: they never overwrite the shipped library
     raise RuntimeError(f'{", ".join(_DIAG)} select a diagnostic build: set S4F_LIB_OUT=<path of the experiment library> as well')
-FILE_DEPS = {'gemm5.hip': ['gemm2.hip'], 'gemm6.hip': ['gemm2.hip']}
+FILE_DEPS = {'gemm5.hip': ['gemm2.hip'], 'gemm6.hip': ['gemm2.hip'], 'qknorm.hip': ['actq8.h'], 'actq8.hip': ['actq8.h'], 'wgradq8.hip': ['actq8.h']}
 
 
 def _hipcc():

@@ -811,12 +811,17 @@ S4F_API int64_t s4f_attention_bwd_ws_bytes(int B, int N, int H) {
   return al256((int64_t)B * H * N * 4) + al256((int64_t)B * H * nchunk * 128 * 4) + al256(nkb * (int64_t)B * N * H * 64 * 4);
 }
 
+int64_t s4f_qk_ws_bytes(int64_t rows, int Hq, int Hk);                           // qknorm.hip
+int64_t s4f_wgrad_packed_ws(const int64_t* dims, int ndims);          // wgradq8.hip
+
 S4F_API int64_t s4f_workspace_bytes(int op, const int64_t* dims, int ndims) {
   if (!dims) return -1;
   switch (op) {
     case S4F_WS_ATTENTION_BWD: return ndims == 3 ? s4f_attention_bwd_ws_bytes((int)dims[0], (int)dims[1], (int)dims[2]) : -1;
     case S4F_WS_BN_SUMS: return ndims == 1 && dims[0] > 0 ? 2 * dims[0] * 4 : -1;
     case S4F_WS_GEMM_SPLITK: return ndims == 2 && dims[0] > 0 && dims[1] > 0 ? dims[0] * dims[1] * 4 : -1;
+    case S4F_WS_QK_NORM: return ndims == 3 && dims[1] <= INT32_MAX && dims[2] <= INT32_MAX ? s4f_qk_ws_bytes(dims[0], (int)dims[1], (int)dims[2]) : -1;
+    case S4F_WS_WGRAD_PACKED: return s4f_wgrad_packed_ws(dims, ndims);
     default: return -1;
   }
 }

@@ -15,7 +15,8 @@ __all__ = ['gemm', 'wgrad_grouped', 'transpose_many', 'cast', 'cast_back', 'im2c
            'layernorm_bwd', 'add_f32', 'attention_fwd', 'attention_bwd', 'attention_bwd_fused', 'attention_bwd_ws_bytes', 'workspace_bytes', 'bn_stats', 'bn_finalize',
            'bn_relu_up_fwd', 'bn_relu_up_bwd', 'bn_bwd_apply', 'bn_param_grads', 'upce_fwd', 'upce_bwd',
            'up_pseudo_label', 'up_logits_nchw', 'ce_fwd', 'ce_bwd', 'ema', 'sgd_momentum', 'ncr_fwd', 'ncr_bwd', 'mix_images',
-           'cutmix_labels', 'gather_rows', 'pasa_patch_u', 'resize_bilinear', 'softmax_argmax', 'confusion_counts']
+           'cutmix_labels', 'gather_rows', 'pasa_patch_u', 'resize_bilinear', 'softmax_argmax', 'confusion_counts',
+           'qk_norm_rope_fwd', 'qk_norm_rope_bwd', 'qk_norm_rope_ws_bytes', 'act_pack', 'act_unpack', 'wgrad_packed', 'wgrad_packed_ws_bytes']
 
 
 def _need(t, n, what):
@@ -474,7 +475,7 @@ def attention_bwd(qkv, ctx, dctx, lse, delta, dqkv, B, N, H, dtype, bias_u=None,
          H, dtype, stream(), tag=('attn', B, N, H))
 
 
-WS_ATTENTION_BWD, WS_BN_SUMS, WS_GEMM_SPLITK = 1, 2, 3
+WS_ATTENTION_BWD, WS_BN_SUMS, WS_GEMM_SPLITK, WS_QK_NORM, WS_WGRAD_PACKED = 1, 2, 3, 4, 5
 
 
 def workspace_bytes(op, *dims):
@@ -505,6 +506,204 @@ def attention_bwd_fused(qkv, ctx, dctx, lse, delta, dqkv, B, N, H, ws, bias_u=No
     nbytes = ws.numel() * ws.element_size()
     call('s4f_attention_bwd_fused', p(qkv), p(ctx), p(dctx), p(lse), p(delta), p(dqkv), p(bias_u), p(row_flag), bias_w, B, N,
          H, p(ws), nbytes, stream(), tag=('attn', B, N, H))
+
+
+# ------------------------------------------------------------------------------------------------ norm + rotation of queries and keys
+def _here(t):
+    return t.is_cuda and t.get_device() == L._cur_device()
+
+
+def _mat(t, dtype, cols, what):
+    """[rows, cols] device matrix, possibly a column slice of a wider buffer -> (pointer, row stride in elements).  A single row has
+    no stride worth the name (torch may report any)."""
+    if t.dim() != 2 or t.shape[1] != cols or t.dtype != dtype:
+        raise S4FError(f'{what}: expected a [rows, {cols}] {dtype} matrix, got {tuple(t.shape)} {t.dtype}')
+    if not _here(t):
+        raise S4FError(f'{what}: expected a tensor on the current device')
+    if cols > 1 and t.stride(1) != 1:
+        raise S4FError(f'{what}: the elements of a row must be contiguous')
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else cols
+
+
+def _vec(t, dtype, n, what):
+    """contiguous device tensor of n elements -> pointer (None -> NULL)"""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or not _here(t):
+        raise S4FError(f'{what}: expected a contiguous {dtype} tensor of {n} elements on the current device, got {tuple(t.shape)} {t.dtype}')
+    return t.data_ptr()
+
+
+def _buf(t, need, what):
+    """workspace of at least `need` bytes -> (pointer, bytes)"""
+    if need == 0:
+        return None, 0
+    if t is None or not t.is_contiguous() or not _here(t) or t.numel() * t.element_size() < need:
+        raise S4FError(f'{what}: expected a contiguous workspace of at least {need} bytes on the current device')
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+def _apart(pa, lda, pb, ldb, rows, row_bytes, es, what):
+    """the two [rows, row_bytes] matrices are the same one, or no element of one lies in the other"""
+    if pa == pb and lda == ldb:
+        return
+    lda, ldb = lda * es, ldb * es
+    if pa + (rows - 1) * lda + row_bytes <= pb or pb + (rows - 1) * ldb + row_bytes <= pa:
+        return
+    if lda == ldb and lda >= 2 * row_bytes and row_bytes <= (pb - pa) % lda <= lda - row_bytes:
+        return                                              # two column slices of one buffer
+    raise S4FError(f'{what} overlap')
+
+
+def _qk_common(x, rows, heads, gq, gk, cos, sin, what):
+    if (gq is None) != (gk is None) or (cos is None) != (sin is None):
+        raise S4FError(f'{what}: gains (gq, gk) and tables (cos, sin) come in pairs')
+    if gq is None and cos is None:
+        raise S4FError(f'{what}: neither a norm (gq, gk) nor a rotation (cos, sin) asked for')
+    period = 0
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape[1] != 32 or cos.shape != sin.shape:
+            raise S4FError(f'{what}: cos and sin must be [positions, 32]')
+        period = cos.shape[0]
+        if period == 0 or rows % period:
+            raise S4FError(f'{what}: {period} positions do not divide {rows} rows')
+    f32 = torch.float32
+    return (_vec(gq, f32, 64, what + ' gq'), _vec(gk, f32, 64, what + ' gk'), _vec(cos, f32, period * 32, what + ' cos'),
+            _vec(sin, f32, period * 32, what + ' sin'), period)
+
+
+def _packed_ptrs(packed, rows, C, what):
+    codes, scales = packed
+    return _vec(codes, torch.int8, rows * C, what + ' codes'), _vec(scales, torch.uint8, rows * (C // 32), what + ' scales')
+
+
+def qk_norm_rope_fwd(x, y, Hq, Hk, dtype, gq=None, gk=None, cos=None, sin=None, eps=1e-6, packed=None):
+    """y[rows, (Hq + Hk) 64] = the query and key heads of x, RMS-normed per head with the gains gq / gk [64] (if given) and turned by the
+    angles of their rows (cos, sin [positions, 32], if given; row r has position r % positions).  x and y may be column slices of
+    wider buffers, and the same one.  packed: (codes int8 [rows, (Hq + Hk) 64], scales uint8 [rows, (Hq + Hk) 2]) receive the 8-bit
+    checkpoint of the pre-norm x that qk_norm_rope_bwd reads."""
+    C, rows, T = (Hq + Hk) * 64, x.shape[0], _tdt(dtype)
+    xp, ldx = _mat(x, T, C, 'qk_norm_rope_fwd x')
+    yp, ldy = _mat(y, T, C, 'qk_norm_rope_fwd y')
+    if y.shape[0] != rows:
+        raise S4FError(f'qk_norm_rope_fwd: x has {rows} rows, y {y.shape[0]}')
+    if packed is not None and gq is None:
+        raise S4FError('qk_norm_rope_fwd: the rotation alone needs no checkpoint')
+    if rows == 0:
+        return
+    gqp, gkp, cp, sp, period = _qk_common(x, rows, Hq + Hk, gq, gk, cos, sin, 'qk_norm_rope_fwd')
+    codes, scales = _packed_ptrs(packed, rows, C, 'qk_norm_rope_fwd') if packed is not None else (None, None)
+    es = x.element_size()
+    _apart(xp, ldx, yp, ldy, rows, C * es, es, 'qk_norm_rope_fwd: x and y')
+    call('s4f_qk_norm_rope_fwd', xp, ldx, yp, ldy, gqp, gkp, cp, sp, period, eps, codes, scales, rows, Hq, Hk, dtype, stream())
+
+
+def qk_norm_rope_ws_bytes(rows, Hq, Hk):
+    return workspace_bytes(WS_QK_NORM, rows, Hq, Hk) if rows else 0
+
+
+def qk_norm_rope_bwd(dy, dx, Hq, Hk, dtype, x=None, packed=None, gq=None, gk=None, cos=None, sin=None, eps=1e-6, dgq=None, dgk=None,
+                     ws=None, accumulate=True):
+    """Backward of qk_norm_rope_fwd: dx from dy (dx may be dy) and, with the norm, the pre-norm x or its checkpoint `packed`; the
+    gain gradients are added to dgq / dgk fp32 [64] (accumulate=False: written).  ws: qk_norm_rope_ws_bytes(rows, Hq, Hk) bytes."""
+    C, rows, T = (Hq + Hk) * 64, dy.shape[0], _tdt(dtype)
+    dyp, lddy = _mat(dy, T, C, 'qk_norm_rope_bwd dy')
+    dxp, lddx = _mat(dx, T, C, 'qk_norm_rope_bwd dx')
+    if dx.shape[0] != rows:
+        raise S4FError(f'qk_norm_rope_bwd: dy has {rows} rows, dx {dx.shape[0]}')
+    if gq is not None and ((x is None) == (packed is None) or dgq is None or dgk is None):
+        raise S4FError('qk_norm_rope_bwd: the norm needs x or packed (not both), dgq and dgk')
+    f32 = torch.float32
+    dgqp, dgkp = (_vec(dgq, f32, 64, 'qk_norm_rope_bwd dgq'), _vec(dgk, f32, 64, 'qk_norm_rope_bwd dgk')) if gq is not None else (None, None)
+    if dgqp is not None and dgqp == dgkp:
+        raise S4FError('qk_norm_rope_bwd: dgq and dgk overlap')
+    if rows == 0:
+        if gq is not None and not accumulate:
+            dgq.zero_(); dgk.zero_()
+        return
+    gqp, gkp, cp, sp, period = _qk_common(dy, rows, Hq + Hk, gq, gk, cos, sin, 'qk_norm_rope_bwd')
+    es = dy.element_size()
+    _apart(dyp, lddy, dxp, lddx, rows, C * es, es, 'qk_norm_rope_bwd: dy and dx')
+    xp, ldx, codes, scales, wsp, wsb = None, 0, None, None, None, 0
+    if gq is not None:
+        if packed is not None:
+            codes, scales = _packed_ptrs(packed, rows, C, 'qk_norm_rope_bwd')
+        else:
+            xp, ldx = _mat(x, T, C, 'qk_norm_rope_bwd x')
+            if x.shape[0] != rows:
+                raise S4FError(f'qk_norm_rope_bwd: dy has {rows} rows, x {x.shape[0]}')
+            _apart(xp, ldx, dxp, lddx, rows, C * es, es, 'qk_norm_rope_bwd: x and dx')
+        wsp, wsb = _buf(ws, qk_norm_rope_ws_bytes(rows, Hq, Hk), 'qk_norm_rope_bwd ws')
+    call('s4f_qk_norm_rope_bwd', dyp, lddy, xp, ldx, codes, scales, dxp, lddx, gqp, gkp, cp, sp, period, eps, dgqp, dgkp,
+         1 if accumulate else 0, wsp, wsb, rows, Hq, Hk, dtype, stream())
+
+
+# ------------------------------------------------------------------------------------------------ activation checkpoints in 8 bits
+def _group_cols(C, what):
+    if C <= 0 or C % 32:
+        raise S4FError(f'{what}: {C} channels are not a positive multiple of 32')
+
+
+def act_pack(x, codes, scales, dtype):
+    """8-bit checkpoint of x [rows, C] (C a multiple of 32; a column slice of a wider buffer qualifies): codes int8 [rows, C], scales uint8
+    [rows, C / 32].  |x - restored| <= max |x| / 127.5 over the 32 channels; a group with an infinity or a NaN comes
+    back as NaN."""
+    C = x.shape[-1]
+    _group_cols(C, 'act_pack')
+    xp, ldx = _mat(x, _tdt(dtype), C, 'act_pack x')
+    rows = x.shape[0]
+    cp, sp = _packed_ptrs((codes, scales), rows, C, 'act_pack')
+    if rows:
+        call('s4f_act_pack', xp, ldx, cp, sp, rows, C, dtype, stream())
+
+
+def act_unpack(codes, scales, y, dtype):
+    """y [rows, C] = the activation that act_pack put away"""
+    C = y.shape[-1]
+    _group_cols(C, 'act_unpack')
+    yp, ldy = _mat(y, _tdt(dtype), C, 'act_unpack y')
+    rows = y.shape[0]
+    cp, sp = _packed_ptrs((codes, scales), rows, C, 'act_unpack')
+    if rows:
+        call('s4f_act_unpack', cp, sp, yp, ldy, rows, C, dtype, stream())
+
+
+def wgrad_packed_ws_bytes(problems, dtype):
+    """problems: (M, N, rows) of each weight gradient of one wgrad_packed call"""
+    return workspace_bytes(WS_WGRAD_PACKED, dtype, *[v for pr in problems if pr[2] for v in pr]) if any(pr[2] for pr in problems) else 0
+
+
+def wgrad_packed(problems, dtype, ws=None, accumulate=True):
+    """problems: up to 4 tuples (dy [rows, M], codes int8 [rows, N], scales uint8 [rows, N / 32], out fp32 [M, N]); out += dy^T x
+    (accumulate=False: out =) with x the restored checkpoint.  M a multiple of 8, N of 32.  One launch for all of them, a second
+    one where the rows are split.  ws: wgrad_packed_ws_bytes([(M, N, rows), ...], dtype) bytes."""
+    if not 1 <= len(problems) <= 4:
+        raise S4FError('wgrad_packed: 1..4 problems')
+    T = _tdt(dtype)
+    descs, dims, spans = [], [], []
+    for dy, codes, scales, out in problems:
+        if out.dim() != 2 or out.shape[0] % 8 or out.shape[1] % 32 or out.shape[0] == 0 or out.shape[1] == 0:
+            raise S4FError(f'wgrad_packed: out must be [M, N] with M a multiple of 8 and N of 32, got {tuple(out.shape)}')
+        M, N = out.shape
+        dyp, ld = _mat(dy, T, M, 'wgrad_packed dy')
+        rows = dy.shape[0]
+        cp, sp = _packed_ptrs((codes, scales), rows, N, 'wgrad_packed')
+        op = _vec(out, torch.float32, M * N, 'wgrad_packed out')
+        spans.append((op, op + 4 * M * N))
+        if rows:
+            descs.append((dyp, ld, cp, sp, op, rows, M, N))
+            dims += [M, N, rows]
+        elif not accumulate:
+            out.zero_()
+    if len(spans) > 1:
+        spans.sort()
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise S4FError('wgrad_packed: the outputs overlap')
+    if not descs:
+        return
+    wsp, wsb = _buf(ws, workspace_bytes(WS_WGRAD_PACKED, dtype, *dims), 'wgrad_packed ws')
+    arr = (L.WgradPackedDesc * len(descs))(*descs)
+    call('s4f_wgrad_packed', arr, len(descs), dtype, 1 if accumulate else 0, wsp, wsb, stream())
 
 
 def bn_stats(x, rows, C, sums, dtype):

@@ -1,0 +1,130 @@
+"""Refusals of the query / key norm and of the 8-bit checkpoints, without a GPU: the typed front's, and the C entry points' (which check
+before anything is launched)."""
+import pytest
+import torch
+
+from s4former_amd import _lib as L
+from s4former_amd import kernels as K
+from s4former_amd._lib import S4FError
+
+P = 1 << 20            # stands for an aligned device address: refused calls never read it
+
+
+def refused(name, args, match):
+    lib = L.load()
+    assert getattr(lib, name)(*args) != 0
+    msg = lib.s4f_last_error().decode()
+    assert match in msg, msg
+
+
+FWD = dict(x=P, ldx=128, y=P, ldy=128, gq=P, gk=P, cos=P, sin=P, period=4, eps=1e-6, codes=None, scales=None, rows=8, Hq=1, Hk=1, dtype=1, stream=None)
+BWD = dict(dy=P, lddy=128, x=P, ldx=128, codes=None, scales=None, dx=P, lddx=128, gq=P, gk=P, cos=P, sin=P, period=4, eps=1e-6, dgq=P, dgk=P,
+           accumulate=0, ws=P, ws_bytes=1 << 20, rows=8, Hq=1, Hk=1, dtype=1, stream=None)
+
+
+@pytest.mark.parametrize('change,match', [
+    (dict(dtype=2), 'dtype'), (dict(rows=0), 'positive'), (dict(Hq=0), 'positive'), (dict(Hk=-1), 'positive'),
+    (dict(rows=1 << 31, period=1 << 31), '2^31'), (dict(gk=None), 'pairs'), (dict(sin=None), 'pairs'),
+    (dict(gq=None, gk=None, cos=None, sin=None), 'neither'), (dict(eps=0.0), 'eps'), (dict(eps=float('nan')), 'eps'), (dict(eps=float('inf')), 'eps'),
+    (dict(period=3), 'divide'), (dict(period=0), 'divide'), (dict(period=16), 'divide'), (dict(x=None), 'null'), (dict(y=None), 'null'),
+    (dict(x=P + 2), '16-byte'), (dict(ldx=129), '16-byte'), (dict(ldy=130), '16-byte'), (dict(ldy=120), 'overlap'), (dict(gq=P + 4), 'aligned'),
+    (dict(cos=P + 8), 'aligned'), (dict(codes=P), 'checkpoint'), (dict(scales=P), 'checkpoint'), (dict(codes=P + 8, scales=P), 'alignment'),
+    (dict(codes=P, scales=P + 1), 'alignment'), (dict(gq=None, gk=None, codes=P, scales=P), 'checkpoint'),
+])
+def test_forward_entry_refuses(change, match):
+    refused('s4f_qk_norm_rope_fwd', {**FWD, **change}.values(), match)
+
+
+@pytest.mark.parametrize('change,match', [
+    (dict(dtype=-1), 'dtype'), (dict(rows=-5), 'positive'), (dict(gq=None), 'pairs'), (dict(period=5), 'divide'), (dict(dy=None), 'null'),
+    (dict(dx=P + 8), '16-byte'), (dict(lddx=64), 'overlap'), (dict(x=None), 'not both'), (dict(codes=P, scales=P), 'not both'),
+    (dict(x=None, codes=P), 'not both'), (dict(ldx=-128), '16-byte'), (dict(dgq=None), 'workspace'), (dict(ws=None), 'workspace'),
+    (dict(ws=P + 4), 'workspace'), (dict(ws_bytes=8), 'too small'),
+])
+def test_backward_entry_refuses(change, match):
+    refused('s4f_qk_norm_rope_bwd', {**BWD, **change}.values(), match)
+
+
+PACK = dict(x=P, ldx=64, codes=P, scales=P, rows=4, C=64, dtype=1, stream=None)
+
+
+@pytest.mark.parametrize('change,match', [
+    (dict(dtype=7), 'dtype'), (dict(x=None), 'null'), (dict(codes=None), 'null'), (dict(scales=None), 'null'), (dict(rows=0), 'positive'),
+    (dict(C=0), '32'), (dict(C=48), '32'), (dict(C=-32), '32'), (dict(x=P + 2), '16-byte'), (dict(ldx=68), '16-byte'), (dict(ldx=-64), '16-byte'),
+    (dict(codes=P + 4), '16-byte'), (dict(rows=1 << 50), 'too large'), (dict(ldx=128, rows=1 << 31), 'too large'),
+])
+def test_pack_entries_refuse(change, match):
+    a = {**PACK, **change}
+    refused('s4f_act_pack', a.values(), match)
+    refused('s4f_act_unpack', (a['codes'], a['scales'], a['x'], a['ldx'], a['rows'], a['C'], a['dtype'], None), match)
+
+
+def test_unpack_entry_refuses_overlapping_rows():
+    refused('s4f_act_unpack', (P, P, P, 32, 4, 64, 1, None), 'overlap')
+
+
+WG = dict(dy=P, lddy=64, codes=P, scales=P, out=P, rows=4096, M=64, N=64)
+
+
+@pytest.mark.parametrize('change,match', [
+    (dict(dy=None), 'null'), (dict(codes=None), 'null'), (dict(scales=None), 'null'), (dict(out=None), 'null'), (dict(M=12), 'multiple'),
+    (dict(N=40), 'multiple'), (dict(M=0), 'multiple'), (dict(rows=0), 'multiple'), (dict(lddy=68), '16-byte'), (dict(dy=P + 8), '16-byte'),
+    (dict(out=P + 4), '16-byte'), (dict(rows=1 << 40), 'too large'), (dict(M=1 << 20, N=1 << 20), 'too large'), (dict(), 'workspace'),
+])
+def test_wgrad_entry_refuses(change, match):
+    good, bad = L.WgradPackedDesc(**WG), L.WgradPackedDesc(**{**WG, **change})
+    arr = (L.WgradPackedDesc * 2)(good, bad)
+    refused('s4f_wgrad_packed', (arr, 2, 1, 0, None, 0, None), match)
+
+
+def test_wgrad_entry_refuses_counts():
+    arr = (L.WgradPackedDesc * 5)(*[L.WgradPackedDesc(**WG)] * 5)
+    for n in (0, 5, -1):
+        refused('s4f_wgrad_packed', (arr, n, 1, 0, P, 1 << 30, None), 'problems')
+    refused('s4f_wgrad_packed', (None, 1, 1, 0, P, 1 << 30, None), 'problems')
+    refused('s4f_wgrad_packed', (arr, 1, 3, 0, P, 1 << 30, None), 'dtype')
+
+
+def test_workspace_queries():
+    assert K.qk_norm_rope_ws_bytes(0, 1, 1) == 0 and K.wgrad_packed_ws_bytes([(8, 32, 0)], 1) == 0
+    one = K.qk_norm_rope_ws_bytes(1, 1, 1)
+    assert 0 < one <= K.qk_norm_rope_ws_bytes(1000, 12, 12) <= K.qk_norm_rope_ws_bytes(1 << 20, 16, 16)
+    assert K.wgrad_packed_ws_bytes([(8, 32, 1)], 1) == 0                          # one range of rows: no slabs
+    for bad in ([(12, 32, 5)], [(8, 33, 5)], [(8, 32, -1)], [(8, 32, 5)] * 5):
+        with pytest.raises(S4FError):
+            K.wgrad_packed_ws_bytes(bad, 1)
+    with pytest.raises(S4FError):
+        K.workspace_bytes(K.WS_QK_NORM, 4, 0, 1)
+
+
+def test_front_refuses():
+    """what the typed front says before a pointer is taken: shapes, types, host tensors"""
+    z = torch.zeros
+    i8, u8, g = lambda *s: z(*s, dtype=torch.int8), lambda *s: z(*s, dtype=torch.uint8), z(64)          # noqa: E731
+    for call in (
+        lambda: K.act_pack(z(4, 64), i8(4, 64), u8(4, 2), 0),                                            # host tensors
+        lambda: K.act_pack(z(4, 48), i8(4, 48), u8(4, 1), 0),
+        lambda: K.act_pack(z(4, 64), i8(4, 64), u8(4, 2), 1),                                            # fp32 tensor, bf16 asked
+        lambda: K.act_pack(z(4, 2, 32), i8(4, 64), u8(4, 2), 0),
+        lambda: K.act_unpack(i8(4, 64), u8(4, 2), z(4, 0), 0),
+        lambda: K.qk_norm_rope_fwd(z(4, 128), z(4, 128), 1, 1, 0, gq=g, gk=g),
+        lambda: K.qk_norm_rope_fwd(z(4, 192), z(4, 128), 1, 1, 0, gq=g, gk=g),
+        lambda: K.qk_norm_rope_bwd(z(4, 128), z(4, 128), 1, 1, 0, x=z(4, 128), gq=g, gk=g, dgq=g, dgk=g),
+        lambda: K.wgrad_packed([], 0),
+        lambda: K.wgrad_packed([(z(4, 8), i8(4, 32), u8(4, 1), z(8, 33))], 0),
+        lambda: K.wgrad_packed([(z(4, 8), i8(4, 32), u8(4, 1), z(8, 32))], 0),
+        lambda: K.wgrad_packed([(z(4, 8), i8(4, 32), u8(4, 1), z(8, 32))] * 5, 0),
+    ):
+        with pytest.raises(S4FError):
+            call()
+
+
+def test_overlap_rule():
+    ap = lambda *a: K._apart(*a, 'x and y')                                                              # noqa: E731
+    ap(1000, 64, 1000, 64, 4, 128, 2)                       # the same matrix
+    ap(0, 64, 512, 64, 4, 128, 2)                           # one behind the other
+    ap(0, 192, 128, 192, 4, 128, 2)                         # neighbouring column slices of one buffer
+    ap(0, 192, 256, 192, 4, 128, 2)
+    for pb, ldb in ((2, 64), (128, 64), (64, 192), (0, 128), (384 - 64, 192)):
+        with pytest.raises(S4FError):
+            ap(0, 192 if ldb == 192 else 64, pb, ldb, 4, 128, 2)
