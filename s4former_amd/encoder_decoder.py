@@ -312,6 +312,8 @@ class EncoderDecoder(BaseSegmentor):
             if s_sig != self._teacher_store.layout_signature():
                 raise S4FError('teacher and student arenas do not line up (backbone_ema/decode_head_ema must mirror '
                                'backbone/decode_head)')
+            if getattr(self.backbone, 'rope_theta', None) != getattr(self.backbone_ema, 'rope_theta', None):
+                raise S4FError('backbone and backbone_ema rotate queries and keys differently (rope_theta)')
 
     def ensure_engine(self, device):
         """(re)build the flat arenas after the model has been moved to `device`; refresh bf16 shadows if stale."""

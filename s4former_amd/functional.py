@@ -465,13 +465,83 @@ def _plan_backward_ready(plan, store, prm, code, dev):
     return plan['event']
 
 
+# ============================================================================================== options of the encoder layer
+class LayerOpt:
+    """What an encoder layer does beyond the reference's: norm - RMS norm of queries and keys per head (two gain parameters behind the
+    layer's twelve); cos, sin - rotation of queries and keys by the position of their token ([tokens, 32] tables); q8 - the activations
+    that only the backward pass reads are kept in 8 bits (kernels.act_pack) instead of their own type."""
+    __slots__ = ('norm', 'cos', 'sin', 'q8')
+
+    def __init__(self, norm=False, cos=None, sin=None, q8=False):
+        self.norm, self.cos, self.sin, self.q8 = norm, cos, sin, q8
+
+    @property
+    def qk(self):
+        return self.norm or self.cos is not None
+
+
+class Packed:
+    """an activation put away in 8 bits; restore() brings it back in its own type and shape"""
+    __slots__ = ('codes', 'scales', 'shape', 'dtype')
+
+    def __init__(self, t):
+        self.shape, self.dtype = t.shape, t.dtype
+        m = t.view(-1, t.shape[-1])
+        self.codes = torch.empty(m.shape, device=t.device, dtype=torch.int8)
+        self.scales = torch.empty(m.shape[0], m.shape[1] // 32, device=t.device, dtype=torch.uint8)
+        K.act_pack(m, self.codes, self.scales, K._xcode(t))
+
+    def restore(self):
+        out = torch.empty(self.shape, device=self.codes.device, dtype=self.dtype)
+        K.act_unpack(self.codes, self.scales, out.view(-1, self.shape[-1]), K._xcode(out))
+        return out
+
+
+def _restored(t):
+    return t.restore() if isinstance(t, Packed) else t
+
+
+def _project_qk(xn, w, b, qkv, M, E, H, code, eps, opt, gq, gk, store, keep):
+    """qkv [M, 3 E] = the projection of xn with queries and keys normed / turned; returns what their backward reads: None, the pre-norm
+    queries and keys, or (8-bit checkpoints) their codes and scales.  With a checkpoint, or when nothing is kept, the projection is one
+    GEMM and the norm works in place; else queries and keys go to a tensor of their own, values straight to their place in qkv (no
+    copy of the pre-norm tensor is made either way)."""
+    par = dict(gq=store.phys(gq) if opt.norm else None, gk=store.phys(gk) if opt.norm else None, cos=opt.cos, sin=opt.sin, eps=eps)
+    qk = qkv[:, :2 * E]
+    wt = store.shadow(w)
+    if keep and opt.norm and not opt.q8:
+        pre = torch.empty(M, 2 * E, device=qkv.device, dtype=qkv.dtype)
+        K.gemm(xn, wt[:2 * E * E], M, 2 * E, E, E, E, code, bias=b[:2 * E], out_t=pre, ldo_t=2 * E)
+        K.gemm(xn, wt[2 * E * E:], M, E, E, E, E, code, bias=b[2 * E:], out_t=qkv.view(-1)[2 * E:], ldo_t=3 * E)
+        K.qk_norm_rope_fwd(pre, qk, H, H, code, **par)
+        return pre
+    K.gemm(xn, wt, M, 3 * E, E, E, E, code, bias=b, out_t=qkv, ldo_t=3 * E)
+    packed = None
+    if keep and opt.norm:
+        packed = (torch.empty(M, 2 * E, device=qkv.device, dtype=torch.int8), torch.empty(M, E // 16, device=qkv.device, dtype=torch.uint8))
+    K.qk_norm_rope_fwd(qk, qk, H, H, code, packed=packed, **par)
+    return packed
+
+
+def _project_qk_bwd(dqkv, pre, M, E, H, code, eps, opt, gq, gk, store):
+    """gradient of queries and keys in dqkv [M, 3 E] -> of the projection's outputs, in place; the gains' gradients into the arena"""
+    dqk = dqkv[:, :2 * E]
+    kw = {}
+    if opt.norm:
+        kw = dict(gq=store.phys(gq), gk=store.phys(gk), dgq=store.grad_phys(gq), dgk=store.grad_phys(gk),
+                  ws=torch.empty(K.qk_norm_rope_ws_bytes(M, H, H), device=dqkv.device, dtype=torch.uint8))
+        kw['packed' if isinstance(pre, tuple) else 'x'] = pre
+    K.qk_norm_rope_bwd(dqk, dqk, H, H, code, cos=opt.cos, sin=opt.sin, eps=eps, **kw)
+
+
 # ============================================================================================== encoder layer
 class LayerFn(Function):
     """x [B,N,E] fp32 -> x + MHA(LN1(x)) -> (+ FFN(LN2(.)))   (vit.py:113-127)"""
 
     @staticmethod
-    def forward(ctx, x, bias_u, row_flag, bias_w, num_heads, eps, store, *prm):
-        (g1, b1, wqkv, bqkv, wo, bo, g2, b2, w1, bf1, w2, bf2) = prm
+    def forward(ctx, x, bias_u, row_flag, bias_w, num_heads, eps, store, opt, *prm):
+        (g1, b1, wqkv, bqkv, wo, bo, g2, b2, w1, bf1, w2, bf2) = prm[:12]
+        gq, gk = prm[12:] if opt is not None and opt.norm else (None, None)
         code = store.dtype
         T = _T(code)
         Bn, N, E = x.shape
@@ -490,10 +560,12 @@ class LayerFn(Function):
         xn2 = torch.empty(M, E, device=dev, dtype=T)
         mean2 = torch.empty(M, device=dev); rstd2 = torch.empty(M, device=dev)
         # gelu'(z) is written only when a backward pass will read it (never on the teacher / inference path)
-        z = torch.empty(M, F_, device=dev, dtype=torch.uint8 if (GELU_Q8 and code == BF16) else T) if need_grad else None
+        q8 = opt is not None and opt.q8 and need_grad
+        z = torch.empty(M, F_, device=dev, dtype=torch.uint8 if ((GELU_Q8 or q8) and code == BF16) else T) if need_grad else None
         a = torch.empty(M, F_, device=dev, dtype=T)
         x2 = torch.empty(Bn, N, E, device=dev, dtype=R)
-        plan = _layer_plan(store, prm, M, E, F_, num_heads, code, R) if (FUSED_LAUNCH and L._prof is None) else None
+        plan = _layer_plan(store, prm, M, E, F_, num_heads, code, R) if (FUSED_LAUNCH and L._prof is None and opt is None) else None
+        pre = None
         if plan is not None:
             d = plan['desc']
             d.B, d.N, d.eps, d.bias_w = Bn, N, eps, float(bias_w)
@@ -504,7 +576,10 @@ class LayerFn(Function):
             L.call('s4f_encoder_layer_fwd', d, L.stream())
         else:
             K.layernorm_fwd(x, store.phys(g1), store.phys(b1), xn, mean1, rstd1, M, E, code, eps)
-            K.gemm(xn, store.shadow(wqkv), M, 3 * E, E, E, E, code, bias=store.phys(bqkv), out_t=qkv, ldo_t=3 * E)
+            if opt is not None and opt.qk:
+                pre = _project_qk(xn, wqkv, store.phys(bqkv), qkv, M, E, num_heads, code, eps, opt, gq, gk, store, need_grad)
+            else:
+                K.gemm(xn, store.shadow(wqkv), M, 3 * E, E, E, E, code, bias=store.phys(bqkv), out_t=qkv, ldo_t=3 * E)
             K.attention_fwd(qkv, ctxv, lse, Bn, N, num_heads, code, bias_u=bias_u, row_flag=row_flag, bias_w=bias_w)
             _gemm_resid(ctxv, store.shadow(wo), M, E, E, code, store.phys(bo), x, x1)
             K.layernorm_fwd(x1, store.phys(g2), store.phys(b2), xn2, mean2, rstd2, M, E, code, eps)
@@ -515,9 +590,14 @@ class LayerFn(Function):
             ctx.store, ctx.prm = store, prm
             ctx.range = store.range_of(prm)
             store.range_acquire(ctx.range)
-            ctx.cfg = (Bn, N, E, F_, num_heads, bias_w)
+            ctx.cfg = (Bn, N, E, F_, num_heads, bias_w, eps, opt)
+            if q8:
+                # queries, keys and values stay in T: the attention backward recomputes the scores, and probabilities of perturbed
+                # scores no longer sum to one against the saved log-sum-exp.  Statistics stay fp32
+                x, xn, ctxv, x1, xn2, a = (Packed(t) for t in (x, xn, ctxv, x1, xn2, a))
+                z = z if code == BF16 else Packed(z)
             ctx.sv = dict(x=x, xn=xn, mean1=mean1, rstd1=rstd1, qkv=qkv, ctxv=ctxv, lse=lse, x1=x1, xn2=xn2, mean2=mean2,
-                          rstd2=rstd2, z=z, a=a, bias_u=bias_u, row_flag=row_flag)
+                          rstd2=rstd2, z=z, a=a, bias_u=bias_u, row_flag=row_flag, pre=pre)
         return x2
 
     @staticmethod
@@ -525,9 +605,13 @@ class LayerFn(Function):
         store = ctx.store
         code = store.dtype
         T = _T(code)
-        (gm1, b1, wqkv, bqkv, wo, bo, gm2, b2, w1, bf1, w2, bf2) = ctx.prm
-        Bn, N, E, F_, H, bias_w = ctx.cfg
+        (gm1, b1, wqkv, bqkv, wo, bo, gm2, b2, w1, bf1, w2, bf2) = ctx.prm[:12]
+        Bn, N, E, F_, H, bias_w, eps, opt = ctx.cfg
+        gq, gk = ctx.prm[12:] if opt is not None and opt.norm else (None, None)
+        q8 = opt is not None and opt.q8
         sv = ctx.sv
+        if sv is None:
+            raise S4FError('backward of an encoder layer a second time: its saved activations are gone')
         M = Bn * N
         dev = g2.device
         g2 = g2.contiguous()
@@ -547,7 +631,7 @@ class LayerFn(Function):
         g0 = torch.empty(Bn, N, E, device=dev, dtype=R)
         g0t = torch.empty(Bn, N, E, device=dev, dtype=T) if (code == BF16 and R != T) else None
         g0cs = zeros_small(E, dev)
-        plan = _layer_plan(store, ctx.prm, M, E, F_, H, code, R) if (FUSED_LAUNCH and L._prof is None) else None
+        plan = _layer_plan(store, ctx.prm, M, E, F_, H, code, R) if (FUSED_LAUNCH and L._prof is None and opt is None) else None
         if plan is not None:
             ev = _plan_backward_ready(plan, store, ctx.prm, code, dev)
             d = plan['desc']
@@ -577,7 +661,7 @@ class LayerFn(Function):
             else:
                 store.grad_phys(bf2).add_(g2cs)
             # (the fc1 bias gradient = column sums of dz comes out of the GEMM's staged output tile where the variant allows)
-            folded = _dgrad(g2t, w2, M, F_, E, store, code, out_t=dz, ldo_t=F_, aux=sv['z'], ld_aux=F_, act=K.ACT_GELU_BWD,
+            folded = _dgrad(g2t, w2, M, F_, E, store, code, out_t=dz, ldo_t=F_, aux=_restored(sv['z']), ld_aux=F_, act=K.ACT_GELU_BWD,
                             colsum=store.grad_phys(bf1))
             sv['z'] = sv['a'] = None
             if not folded:
@@ -585,24 +669,37 @@ class LayerFn(Function):
                     K.colsum(dz, F_, M, F_, store.grad_phys(bf1), code)
             _dgrad(dz, w1, M, E, F_, store, code, out_t=dxn2, ldo_t=E)
             # the column sums of g1 (= the proj bias gradient) come out of the same pass
-            K.layernorm_bwd(dxn2, sv['x1'], sv['mean2'], sv['rstd2'], store.phys(gm2), g2, g1, g1t if g1t is not g1 else None, store.grad_phys(gm2),
+            K.layernorm_bwd(dxn2, _restored(sv['x1']), sv['mean2'], sv['rstd2'], store.phys(gm2), g2, g1, g1t if g1t is not g1 else None, store.grad_phys(gm2),
                             store.grad_phys(b2), M, E, code, dcolsum=store.grad_phys(bo))
             # ---- attention
             _dgrad(g1t, wo, M, E, E, store, code, out_t=dctx, ldo_t=E)
+            ctx_t = _restored(ctxv)
             if attn_ws is not None:
-                K.attention_bwd_fused(sv['qkv'], sv['ctxv'], dctx, sv['lse'], delta, dqkv, Bn, N, H, attn_ws, bias_u=sv['bias_u'],
+                K.attention_bwd_fused(sv['qkv'], ctx_t, dctx, sv['lse'], delta, dqkv, Bn, N, H, attn_ws, bias_u=sv['bias_u'],
                                       row_flag=sv['row_flag'], bias_w=bias_w)
             else:
-                K.attention_bwd(sv['qkv'], sv['ctxv'], dctx, sv['lse'], delta, dqkv, Bn, N, H, code, bias_u=sv['bias_u'],
+                K.attention_bwd(sv['qkv'], ctx_t, dctx, sv['lse'], delta, dqkv, Bn, N, H, code, bias_u=sv['bias_u'],
                                 row_flag=sv['row_flag'], bias_w=bias_w)
-            with on_side(dev, dqkv, xn, dz, xn2, g1t, ctxv, g2t, a_act, enable=LAYER_WG_SIDE):
-                K.wgrad_grouped([(dz, xn2, F_, E, M, store.grad_phys(w1)),
-                                 (g2t, a_act, E, F_, M, store.grad_phys(w2)),
-                                 (dqkv, xn, 3 * E, E, M, store.grad_phys(wqkv)),
-                                 (g1t, ctxv, E, E, M, store.grad_phys(wo))], code)
-                K.colsum(dqkv, 3 * E, M, 3 * E, store.grad_phys(bqkv), code)
+            del ctx_t
+            if opt is not None and opt.qk:
+                _project_qk_bwd(dqkv, sv['pre'], M, E, H, code, eps, opt, gq, gk, store)
+            if q8:
+                kept = ((dz, xn2, w1), (g2t, a_act, w2), (dqkv, xn, wqkv), (g1t, ctxv, wo))
+                with on_side(dev, *[t for dy, pk, _ in kept for t in (dy, pk.codes, pk.scales)], enable=LAYER_WG_SIDE):
+                    probs = [(dy.view(M, -1), pk.codes, pk.scales, store.grad_phys(w).view(w.shape)) for dy, pk, w in kept]
+                    ws = torch.empty(K.wgrad_packed_ws_bytes([(*w.shape, M) for _, _, w in kept], code), device=dev, dtype=torch.uint8)
+                    K.wgrad_packed(probs, code, ws)
+                    K.colsum(dqkv, 3 * E, M, 3 * E, store.grad_phys(bqkv), code)
+                    del ws, probs
+            else:
+                with on_side(dev, dqkv, xn, dz, xn2, g1t, ctxv, g2t, a_act, enable=LAYER_WG_SIDE):
+                    K.wgrad_grouped([(dz, xn2, F_, E, M, store.grad_phys(w1)),
+                                     (g2t, a_act, E, F_, M, store.grad_phys(w2)),
+                                     (dqkv, xn, 3 * E, E, M, store.grad_phys(wqkv)),
+                                     (g1t, ctxv, E, E, M, store.grad_phys(wo))], code)
+                    K.colsum(dqkv, 3 * E, M, 3 * E, store.grad_phys(bqkv), code)
             _dgrad(dqkv, wqkv, M, E, 3 * E, store, code, out_t=dxn, ldo_t=E)
-            K.layernorm_bwd(dxn, sv['x'], sv['mean1'], sv['rstd1'], store.phys(gm1), g1, g0, g0t, store.grad_phys(gm1),
+            K.layernorm_bwd(dxn, _restored(sv['x']), sv['mean1'], sv['rstd1'], store.phys(gm1), g1, g0, g0t, store.grad_phys(gm1),
                             store.grad_phys(b1), M, E, code, dcolsum=g0cs)
         del dqkv, dz
         # reused by the previous layer if autograd hands this very tensor through unmodified (autograd may
@@ -613,7 +710,7 @@ class LayerFn(Function):
         ctx.sv = None
         store.node_done()
         store.range_release(ctx.range)
-        return (g0,) + (None,) * (6 + 12)
+        return (g0,) + (None,) * (7 + len(ctx.prm))
 
 
 # Round 5: heads advancing in lockstep (MultiHeadLossFn: the four auxiliary heads) issue their same-shape small convs - the

@@ -18,7 +18,7 @@ import torch.nn.functional as F
 from . import runtime
 from ._lib import F32, S4FError
 from .base_module import BaseModule, ModuleList, constant_init, kaiming_init, trunc_normal_
-from .functional import LayerFn, PatchEmbedFn
+from .functional import LayerFn, LayerOpt, PatchEmbedFn
 from .params import ParamStore
 from .registry import BACKBONES
 
@@ -62,13 +62,24 @@ class PatchEmbed(BaseModule):
         return x
 
 
-class _AttnContainer(BaseModule):
-    """mmcv MultiheadAttention wrapper: parameter path `attn.attn.*` (nn.MultiheadAttention container)."""
+class _Gain(BaseModule):
+    """gain of an RMS norm: parameter path `weight`"""
 
-    def __init__(self, embed_dims, num_heads, bias=True):
+    def __init__(self, dims):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(dims))
+
+
+class _AttnContainer(BaseModule):
+    """mmcv MultiheadAttention wrapper: parameter path `attn.attn.*` (nn.MultiheadAttention container); qk_norm adds `attn.q_norm.weight`
+    and `attn.k_norm.weight` [64], shared by the heads."""
+
+    def __init__(self, embed_dims, num_heads, bias=True, qk_norm=False):
         super().__init__()
         self.embed_dims, self.num_heads = embed_dims, num_heads
         self.attn = nn.MultiheadAttention(embed_dims, num_heads, 0.0, bias=bias)
+        if qk_norm:
+            self.q_norm, self.k_norm = _Gain(embed_dims // num_heads), _Gain(embed_dims // num_heads)
         self.self_attn = None       # Q7: the patched mmcv stored head-averaged weights here (visualisation only)
 
 
@@ -84,11 +95,12 @@ class _FFNContainer(BaseModule):
 
 class TransformerEncoderLayer(BaseModule):
     """reference vit.py:28-127.  forward(x, attn_mask) with attn_mask given in the rank-1 form
-    (bias_u [B,N], row_flag [B,N] | None, weight) or None."""
+    (bias_u [B,N], row_flag [B,N] | None, weight) or None.  qk_norm, act_q8 and the rotation tables given to forward are options beyond the
+    reference (VisionTransformer has their description)."""
 
     def __init__(self, embed_dims, num_heads, feedforward_channels, drop_rate=0., attn_drop_rate=0., drop_path_rate=0.,
                  num_fcs=2, qkv_bias=True, act_cfg=dict(type='GELU'), norm_cfg=dict(type='LN'), batch_first=True,
-                 attn_cfg=dict(), ffn_cfg=dict(), with_cp=False):
+                 attn_cfg=dict(), ffn_cfg=dict(), with_cp=False, qk_norm=False, act_q8=False):
         super().__init__()
         if drop_rate or attn_drop_rate or drop_path_rate:
             raise S4FError('dropout / drop-path are 0 in every SETR config; the fused layer has no dropout')
@@ -97,9 +109,10 @@ class TransformerEncoderLayer(BaseModule):
         self.embed_dims, self.num_heads = embed_dims, num_heads
         self.eps = float(norm_cfg.get('eps', 1e-5))
         self.ln1 = nn.LayerNorm(embed_dims, eps=self.eps)
-        self.attn = _AttnContainer(embed_dims, num_heads, bias=qkv_bias)
+        self.attn = _AttnContainer(embed_dims, num_heads, bias=qkv_bias, qk_norm=qk_norm)
         self.ln2 = nn.LayerNorm(embed_dims, eps=self.eps)
         self.ffn = _FFNContainer(embed_dims, feedforward_channels)
+        self.qk_norm, self.act_q8 = bool(qk_norm), bool(act_q8)
         self._store = None
 
     @property
@@ -118,10 +131,11 @@ class TransformerEncoderLayer(BaseModule):
 
     def _build_params(self):
         a, f = self.attn.attn, self.ffn.layers
+        gains = (self.attn.q_norm.weight, self.attn.k_norm.weight) if self.qk_norm else ()
         return (self.ln1.weight, self.ln1.bias, a.in_proj_weight, a.in_proj_bias, a.out_proj.weight, a.out_proj.bias,
-                self.ln2.weight, self.ln2.bias, f[0][0].weight, f[0][0].bias, f[1].weight, f[1].bias)
+                self.ln2.weight, self.ln2.bias, f[0][0].weight, f[0][0].bias, f[1].weight, f[1].bias) + gains
 
-    def forward(self, x, attn_mask=None):
+    def forward(self, x, attn_mask=None, rope=None):
         store = self._store
         if store is None:
             raise S4FError('TransformerEncoderLayer must be run through VisionTransformer (it owns the ParamStore)')
@@ -129,18 +143,42 @@ class TransformerEncoderLayer(BaseModule):
         bw = 0.0
         if attn_mask is not None:
             bu, rf, bw = attn_mask
-        return LayerFn.apply(x, bu, rf, float(bw), self.num_heads, self.eps, store, *self._params())
+        opt = None
+        if self.qk_norm or self.act_q8 or rope is not None:
+            cos, sin = rope if rope is not None else (None, None)
+            opt = LayerOpt(self.qk_norm, cos, sin, self.act_q8)
+        return LayerFn.apply(x, bu, rf, float(bw), self.num_heads, self.eps, store, opt, *self._params())
+
+
+def axial_rope_tables(h, w, theta, device):
+    """cos and sin fp32 [1 + h w, 32] of the rotation of queries and keys on an h x w patch grid: pairs 0..15 of a head turn with the patch's
+    row, pairs 16..31 with its column, by theta^(-i / 16) radians a patch; the cls token is not turned.  Angles in 64 bits."""
+    freq = float(theta) ** (-torch.arange(16, dtype=torch.float64) / 16)
+    y, x = torch.meshgrid(torch.arange(h, dtype=torch.float64), torch.arange(w, dtype=torch.float64), indexing='ij')
+    ang = torch.cat([y.reshape(-1, 1) * freq, x.reshape(-1, 1) * freq], -1)
+    ang = torch.cat([torch.zeros(1, 32, dtype=torch.float64), ang])
+    return ang.cos().float().to(device), ang.sin().float().to(device)
 
 
 @BACKBONES.register_module()
 class VisionTransformer(BaseModule):
-    """reference vit.py:129-577 (DeiT-B / ViT for SETR)."""
+    """reference vit.py:129-577 (DeiT-B / ViT for SETR).
+
+    Options beyond the reference, all off by default (a student and its teacher take the same ones):
+      qk_norm      RMS norm of every query and key head in front of the attention, with a learned gain [64] each for queries and keys
+                   shared by the heads: bounds the attention logits, which bf16 training of larger models needs
+      rope_theta   (e.g. 100.) queries and keys are turned by the row and column of their patch (axial_rope_tables), in addition to
+                   the learned position embedding: attention sees relative positions
+      act_q8       what only the backward pass reads of a layer's activations is kept in 8 bits (kernels.act_pack) and its weight
+                   gradients are computed from that: 17 instead of 32 bytes a token and channel in bf16 mode.  The forward pass is
+                   not changed; gradients carry the rounding of the kept activations."""
 
     def __init__(self, img_size=224, patch_size=16, in_channels=3, embed_dims=768, num_layers=12, num_heads=12, mlp_ratio=4,
                  out_indices=-1, qkv_bias=True, drop_rate=0., attn_drop_rate=0., drop_path_rate=0., with_cls_token=True,
                  output_cls_token=False, norm_cfg=dict(type='LN'), act_cfg=dict(type='GELU'), patch_norm=False,
                  final_norm=False, interpolate_mode='bicubic', num_fcs=2, norm_eval=False, with_cp=False, pretrained=None,
-                 init_cfg=None, no_pos_embed=False, feature_ps_indices=0, w_PatchRelativeAttention=False):
+                 init_cfg=None, no_pos_embed=False, feature_ps_indices=0, w_PatchRelativeAttention=False,
+                 qk_norm=False, rope_theta=None, act_q8=False):
         super().__init__(init_cfg=init_cfg)
         if isinstance(img_size, int):
             img_size = to_2tuple(img_size)
@@ -160,6 +198,11 @@ class VisionTransformer(BaseModule):
             raise S4FError('the patch-embed kernels are built for 16x16 RGB patches')
         if not with_cls_token or patch_norm or w_PatchRelativeAttention or with_cp:
             raise S4FError('with_cls_token=False / patch_norm / PatchRelativeAttention / with_cp are outside the SETR hot path')
+        if rope_theta is not None and not 1.0 <= float(rope_theta) < math.inf:
+            raise S4FError(f'rope_theta must be a finite number of at least 1, got {rope_theta}')
+        self.qk_norm, self.act_q8 = bool(qk_norm), bool(act_q8)
+        self.rope_theta = None if rope_theta is None else float(rope_theta)
+        self._rope_tables = {}       # (h, w, device) -> (cos, sin)
         self.img_size, self.patch_size = tuple(img_size), patch_size
         self.interpolate_mode, self.norm_eval, self.with_cp = interpolate_mode, norm_eval, with_cp
         self.pretrained, self.num_heads, self.embed_dims = pretrained, num_heads, embed_dims
@@ -186,7 +229,8 @@ class VisionTransformer(BaseModule):
         self.layers = ModuleList([
             TransformerEncoderLayer(embed_dims=embed_dims, num_heads=num_heads, feedforward_channels=mlp_ratio * embed_dims,
                                     attn_drop_rate=attn_drop_rate, drop_rate=drop_rate, drop_path_rate=0., num_fcs=num_fcs,
-                                    qkv_bias=qkv_bias, act_cfg=act_cfg, norm_cfg=norm_cfg, with_cp=with_cp, batch_first=True)
+                                    qkv_bias=qkv_bias, act_cfg=act_cfg, norm_cfg=norm_cfg, with_cp=with_cp, batch_first=True,
+                                    qk_norm=qk_norm, act_q8=act_q8)
             for _ in range(num_layers)])
         self.final_norm = final_norm
         if final_norm:
@@ -290,6 +334,14 @@ class VisionTransformer(BaseModule):
             mask = self._rank1_mask(attn_mask, attn_mask_weight, adaptive_attn_mask)
         return self.forward_rank1(inputs, mask)
 
+    def _rope(self, hw, device):
+        if self.rope_theta is None:
+            return None
+        key = (*hw, torch.device(device))
+        if key not in self._rope_tables:
+            self._rope_tables[key] = axial_rope_tables(*hw, self.rope_theta, device)
+        return self._rope_tables[key]
+
     def forward_rank1(self, inputs, mask=None, tap_groups=None):
         """forward with the PASA mask already in rank-1 form (bias_u [B,N], row_flag [B,N] | None, weight) | None.
         The segmentor uses this to push several image groups (supervised, masked / plain unlabeled) through the
@@ -303,11 +355,12 @@ class VisionTransformer(BaseModule):
         pe = self.patch_embed.projection
         tokens = PatchEmbedFn.apply(x, pe.weight, pe.bias, self.cls_token, self.pos_embed, store)
         outs = []
+        rope = self._rope(hw_shape, x.device)
         wait = self.__dict__.pop('_pre_layer_wait', None)   # (layer index, event): the part of this (teacher) model's weights that
         for i, layer in enumerate(self.layers):             # the EMA updates on the side stream (encoder_decoder.update_ema_variables)
             if wait is not None and i == wait[0]:
                 torch.cuda.current_stream().wait_event(wait[1])
-            tokens = layer(tokens, mask)
+            tokens = layer(tokens, mask, rope)
             if i in self.out_indices:
                 parts = None
                 if tap_groups is not None:

@@ -128,3 +128,42 @@ def test_overlap_rule():
     for pb, ldb in ((2, 64), (128, 64), (64, 192), (0, 128), (384 - 64, 192)):
         with pytest.raises(S4FError):
             ap(0, 192 if ldb == 192 else 64, pb, ldb, 4, 128, 2)
+
+
+# ------------------------------------------------------------------------------------------------------------- options of the backbone
+def test_backbone_options():
+    import s4former_amd as S
+    from tests import common as C
+    plain = C.tiny_model_cfg(unsup_weight=1.0)
+    keys = set(S.build_segmentor(plain).state_dict())
+    cfg = C.tiny_model_cfg(unsup_weight=1.0)
+    for k in ('backbone', 'backbone_ema'):
+        cfg[k].update(qk_norm=True, rope_theta=100.0, act_q8=True)
+    m = S.build_segmentor(cfg)
+    more = set(m.state_dict()) - keys
+    assert keys <= set(m.state_dict())
+    assert more == {f'{b}.layers.{i}.attn.{n}_norm.weight' for b in ('backbone', 'backbone_ema') for i in range(4) for n in 'qk'}
+    assert all(tuple(m.state_dict()[k].shape) == (64,) and bool((m.state_dict()[k] == 1).all()) for k in more)
+    m._build_stores()
+    for bad in (0.0, -1.0, 0.5, float('inf'), float('nan')):
+        cfg['backbone']['rope_theta'] = bad
+        with pytest.raises(S4FError):
+            S.build_segmentor(cfg)
+    cfg['backbone']['rope_theta'] = 10.0
+    with pytest.raises(S4FError, match='rope_theta'):
+        S.build_segmentor(cfg)._build_stores()
+    cfg['backbone']['rope_theta'] = 100.0
+    cfg['backbone_ema']['qk_norm'] = False
+    with pytest.raises(S4FError, match='line up'):
+        S.build_segmentor(cfg)._build_stores()
+
+
+def test_axial_tables():
+    from s4former_amd.vit import axial_rope_tables
+    cos, sin = axial_rope_tables(3, 5, 100.0, 'cpu')
+    assert cos.shape == sin.shape == (16, 32) and cos.dtype == torch.float32
+    assert bool((cos[0] == 1).all()) and bool((sin[0] == 0).all())                # the cls token is not turned
+    row, col, i = 2, 4, 5
+    t = 1 + row * 5 + col
+    a, b = torch.tensor(row * 100.0 ** (-i / 16), dtype=torch.float64), torch.tensor(col * 100.0 ** (-i / 16), dtype=torch.float64)
+    assert cos[t, i] == a.cos().float() and sin[t, i] == a.sin().float() and cos[t, 16 + i] == b.cos().float() and sin[t, 16 + i] == b.sin().float()
