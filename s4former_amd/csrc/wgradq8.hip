@@ -24,7 +24,7 @@ struct Problem {
   int M, N, tiles_n, tiles, splits, steps, steps_per_split;
   int work_end;                          // running sum of tiles x splits
 };
-struct Args { Problem p[MAXP]; int count, accumulate; };
+struct Args { Problem p[MAXP]; int count, accumulate, variant; };
 
 // ------------------------------------------------------------------------------------------------- 128 x 128 tile, any type
 constexpr int BT = 128, BKR = 32;
@@ -127,6 +127,276 @@ __global__ __launch_bounds__(256) void wgrad_kernel(const Args args) {
     }
 }
 
+// ------------------------------------------------------------------------------------------------- bf16
+// Tile (64 MI) x (64 NI), four waves in 2 x 2, each MI x NI products of 32 x 32 x 16; 64 rows of dY and X a step, two buffers in LDS.
+// One wave per SIMD holds the sums of a quarter of the tile, so that a fragment read feeds four products (at 256 x 256): with eight
+// waves LDS would bound the loop.  A wave alone on its SIMD has to keep the matrix unit busy by itself, so every read, store and
+// conversion stands between products:
+//   barrier (step k's buffer is complete, the other one free)
+//   part 0: products of step k - 1's last 16 rows, reads of the fragments of step k's rows 0 .. 15
+//   parts 1 - 3: products of 16 rows of step k, reads of the next 16
+// Parts 0 - 2 also store a third each of step k + 1 (in registers since about two steps; codes become bf16 on the way) into the other
+// buffer and load what takes its registers' place; part 3 reads early and stores nothing, so that nothing is left to wait for at
+// the barrier, and the products behind the barrier have their fragments in registers.
+//
+// LDS image: [64 rows][columns] bf16, the 64-byte unit u of row r at u ^ (r & 3): the four rows x 64 bytes that half a wave reads in
+// one transposing read lie in different banks, and so do the stores.
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+constexpr int STEP = 64;
+
+// four rows of 16 columns, transposed (all lanes of the wave take part)
+__device__ __forceinline__ s16x4 tr_read(const char* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+}
+struct Frag8 {                                            // eight rows of a column: two transposed reads
+  s16x4 h[2];
+  __device__ __forceinline__ bf16x8 v() const {
+    union { s16x4 s[2]; bf16x8 b; } u;
+    u.s[0] = h[0]; u.s[1] = h[1];
+    return u.b;
+  }
+};
+
+template <int MI, int NI, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args args) {
+  constexpr int NT = 64 * WM * WN, TM = 32 * MI * WM, TN = 32 * NI * WN, RA = TM * 2, RB = TN * 2;
+  constexpr int CA = TM / 8, CB = TN / 16;                // 16-byte chunks of a row of dY / of codes
+  constexpr int NA = STEP * CA / NT, NB = STEP * CB / NT, DA = NT / CA, DB = NT / CB;      // chunks a thread, rows between them
+  // one object a buffer: the compiler then sees that a read of one does not wait for what arrives in another
+  __shared__ __attribute__((aligned(1024))) char A0[STEP * RA], A1[STEP * RA], B0[STEP * RB], B1[STEP * RB];
+
+  // block -> (problem, row range, tile), consecutive ones on one XCD: the tiles of a row range read the same rows of dY and X
+  const int total = args.p[args.count - 1].work_end;
+  const int xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
+  const int w = min(xcd, r8) * (q8 + 1) + max(xcd - r8, 0) * q8 + (blockIdx.x >> 3);
+  int which = 0;
+  for (int i = 0; i < MAXP - 1; ++i) which += i < args.count - 1 && w >= args.p[i].work_end ? 1 : 0;
+  const Problem& P = args.p[which];
+  const int local = w - (which ? args.p[which - 1].work_end : 0);
+  const int z = local / P.tiles, tile = local - z * P.tiles;
+  const int m0 = tile / P.tiles_n * TM, n0 = tile % P.tiles_n * TN;
+  const int k_beg = z * P.steps_per_split, k_end = min(k_beg + P.steps_per_split, P.steps);
+  const int M = P.M, N = P.N;
+
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63;
+  const int wm = wave / WN, wn = wave % WN;
+
+  // ---- global side: chunk i of a thread is DA (DB) rows below chunk i - 1.  The resources cover the rows of the step, so rows behind
+  // the range read as zero; columns outside are given an offset beyond every resource.  16 codes come as two loads of 8: the lanes
+  // whose chunk lies in the upper 256 bytes of a 512-byte span of LDS take (and store) the upper half first, so that the 16 lanes of
+  // one 16-byte store touch every bank once
+  const int ra = tid / CA, ua = (tid % CA >> 2) ^ (ra & 3), ca = 4 * ua + (tid & 3), rb = tid / CB, cb = tid % CB, hb = (tid >> 2) & 1;
+  const int OUT = (int)0x80000000;
+  const int ld2 = (int)(P.lddy * 2), ns = N / ACTQ8_GROUP;
+  const int va = m0 + 8 * ca < M ? ra * ld2 + (m0 + 8 * ca) * 2 : OUT;
+  const int vb = n0 + 16 * cb < N ? rb * N + n0 + 16 * cb + 8 * hb : OUT, vb2 = vb + 8 - 16 * hb;
+  const int vs = n0 + 16 * cb < N ? rb * ns + (n0 + 16 * cb) / ACTQ8_GROUP : OUT;
+  struct Regs { u32x2 b[NB][2]; uint32_t s[NB]; } R[2];
+  const int64_t r_beg = (int64_t)k_beg * STEP;
+  int left = (int)(min(P.rows, (int64_t)k_end * STEP) - r_beg);
+  int left_a = left;
+  char* pa = (char*)P.dy + r_beg * ld2;
+  char* pb = (char*)P.codes + r_beg * N;
+  char* ps = (char*)P.scales + r_beg * ns;
+  __amdgpu_buffer_rsrc_t qa, qb, qs;
+  auto next_rows = [&]() {                                // the resources of the next step's rows (none left: empty ones)
+    const int nr = __builtin_amdgcn_readfirstlane(max(min(left, STEP), 0));
+    qb = __builtin_amdgcn_make_buffer_rsrc(pb, 0, nr * N, 0x00020000);
+    qs = __builtin_amdgcn_make_buffer_rsrc(ps, 0, nr * ns, 0x00020000);
+    left -= STEP;
+    pb += (int64_t)STEP * N; ps += (int64_t)STEP * ns;
+  };
+  auto next_rows_a = [&]() {
+    const int nr = __builtin_amdgcn_readfirstlane(max(min(left_a, STEP), 0));
+    qa = __builtin_amdgcn_make_buffer_rsrc(pa, 0, nr * ld2, 0x00020000);
+    left_a -= STEP;
+    pa += (int64_t)STEP * ld2;
+  };
+  // a step's chunks of dY and half chunks of codes in three shares
+  constexpr auto a_from = [](int t) { return (t * NA + 2) / 3; };
+  constexpr auto b_from = [](int t) { return t * 2 * NB / 3; };
+  // dY goes to LDS without a stop in registers: 64 lanes x 16 bytes in a row, so the unit's place is chosen on the source side
+  auto load_a = [&](int i, auto bufc) {
+    char* d = (decltype(bufc)::value ? A1 : A0) + (WM * WN * i + wave) * 1024;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(qa, (__attribute__((address_space(3))) void*)d, 16, va + i * DA * ld2, 0, 0, 0);
+  };
+  auto load_b = [&](Regs& r, int i) {                     // half chunk i; the chunk's scale behind its second half
+    r.b[i >> 1][i & 1] = __builtin_amdgcn_raw_buffer_load_b64(qb, ((i & 1) ? vb2 : vb) + (i >> 1) * DB * N, 0, 0);
+    if (i & 1) r.s[i >> 1] = __builtin_amdgcn_raw_buffer_load_b8(qs, vs + (i >> 1) * DB * ns, 0, 0);
+  };
+
+  // ---- LDS side.  DA and DB are multiples of 4: a thread's rows agree in their lower two bits
+  static_assert(DA % 4 == 0 && DB % 4 == 0, "the unit's place depends on the thread alone");
+  const int ob = rb * RB + (((cb >> 1) ^ (rb & 3)) << 6) + (cb & 1) * 32 + 16 * hb, ob2 = ob + 16 - 32 * hb;
+  u32x4 conv;                                             // the half chunk under conversion
+  float cs = 0.f;                                         // and its scale
+  auto convert = [&](const Regs& r, int i, int e, auto bufc) {                   // two codes of half chunk i; the last two store it
+    if (e == 0) cs = q8_scale(r.s[i >> 1]);
+    const uint32_t w = r.b[i >> 1][i & 1][e >> 1];
+    conv[e] = pack_exact_bf16(q8_code(w, 2 * (e & 1)) * cs, q8_code(w, 2 * (e & 1) + 1) * cs);
+    if (e == 3) *reinterpret_cast<u32x4*>((decltype(bufc)::value ? B1 : B0) + ((i & 1) ? ob2 : ob) + (i >> 1) * DB * RB) = conv;
+  };
+
+  // ---- fragments: lane (half, col & 31): 8 rows 8 half .. + 7 of a part.  A transposing read gives 16 lanes a 4 x 16 block
+  const int g = l >> 4, q = (l >> 2) & 3, p4 = l & 3;
+  int fa[MI], fb[NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) fa[i] = (8 * (g >> 1) + q) * RA + (((wm * MI + i) ^ q) << 6) + (g & 1) * 32 + p4 * 8;
+#pragma unroll
+  for (int j = 0; j < NI; ++j) fb[j] = (8 * (g >> 1) + q) * RB + (((wn * NI + j) ^ q) << 6) + (g & 1) * 32 + p4 * 8;
+  struct Frags { Frag8 a[MI], b[NI]; } F[2];
+  auto read = [&](Frags& f, int i, auto bufc, int part) { // read i of 2 (NI + MI)
+    const int row = part * 16 + 4 * (i & 1);
+    if (i < 2 * NI) f.b[i >> 1].h[i & 1] = tr_read((decltype(bufc)::value ? B1 : B0) + fb[i >> 1] + row * RB);
+    else f.a[(i >> 1) - NI].h[i & 1] = tr_read((decltype(bufc)::value ? A1 : A0) + fa[(i >> 1) - NI] + row * RA);
+  };
+  f32x16 acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  auto mma = [&](const Frags& f, int i) {
+    acc[i / NI][i % NI] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a[i / NI].v(), f.b[i % NI].v(), acc[i / NI][i % NI], 0, 0, 0);
+  };
+  auto barrier = [&]() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  };
+  // vector loads of a step behind its loads of dY: the half chunks of shares 1 and 2 and their scales at least
+  constexpr int BEHIND = (2 * NB - b_from(1)) + (NB - b_from(1) / 2);
+  constexpr int WAIT = (BEHIND & 15) | (BEHIND >> 4 << 14) | (7 << 4) | (15 << 8);       // vmcnt(BEHIND), the other counters free
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using I3 = std::integral_constant<int, 3>;
+  // one part: products of f, fragments of (buffer rbuf, part rpart) to n; share T < 3 of r to buffer sbuf, its registers refilled.  The
+  // order is the one written here: a product, then what the matrix unit's 32 cycles leave room for
+  auto part = [&](const Frags& f, Frags& n, auto rbuf, int rpart, Regs& r, auto tc, auto sbuf) {
+    constexpr int T = decltype(tc)::value, P = MI * NI, RD = 2 * (MI + NI), RP = T < 3 ? P : P / 2;
+    constexpr int na = T == 0 ? NA : 0, b0 = T < 3 ? b_from(T) : 0, nc = T < 3 ? 4 * (b_from(T + 1) - b0) : 0;
+    static_for<P>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      mma(f, i);
+#pragma unroll
+      for (int k = std::min(i, RP) * RD / RP; k < std::min(i + 1, RP) * RD / RP; ++k) read(n, k, rbuf, rpart);
+#pragma unroll
+      for (int k = i * na / P; k < (i + 1) * na / P; ++k) load_a(k, sbuf);
+#pragma unroll
+      for (int k = i * nc / P; k < (i + 1) * nc / P; ++k) {
+        convert(r, b0 + k / 4, k % 4, sbuf);
+        if (k % 4 == 3) load_b(r, b0 + k / 4);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  auto step = [&](auto bufc) {
+    constexpr int b = decltype(bufc)::value;
+    using Cur = std::integral_constant<int, b>;
+    using Oth = std::integral_constant<int, b ^ 1>;
+    Regs& r = R[b ^ 1];
+    __builtin_amdgcn_s_waitcnt(WAIT);                     // this wave's dY of the step has arrived (the loads of codes behind it need not have)
+    barrier();
+    next_rows();
+    next_rows_a();
+    part(F[1], F[0], Cur{}, 0, r, I0{}, Oth{});
+    part(F[0], F[1], Cur{}, 1, r, I1{}, Oth{});
+    part(F[1], F[0], Cur{}, 2, r, I2{}, Oth{});
+    part(F[0], F[1], Cur{}, 3, r, I3{}, Oth{});
+  };
+
+  if (k_beg < k_end) {
+    auto load_all = [&](Regs& r) {
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) load_b(r, i);
+    };
+    next_rows_a();
+#pragma unroll
+    for (int i = 0; i < NA; ++i) load_a(i, I0{});
+    next_rows();
+    load_all(R[0]);
+    next_rows();
+    load_all(R[1]);
+#pragma unroll
+    for (int i = 0; i < 8 * NB; ++i) convert(R[0], i / 4, i % 4, I0{});
+    next_rows();
+    load_all(R[0]);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) F[1].a[i] = Frag8{};
+#pragma unroll
+    for (int j = 0; j < NI; ++j) F[1].b[j] = Frag8{};
+    for (int k = k_beg; k < k_end; k += 2) {              // (behind the last step of an odd range: one on zeros)
+      step(I0{});
+      step(I1{});
+    }
+#pragma unroll
+    for (int i = 0; i < MI * NI; ++i) mma(F[1], i);
+    __builtin_amdgcn_s_waitcnt(15 << 8 | 7 << 4);           // nothing arrives in LDS behind the wave's end: vmcnt(0)
+  }
+
+  // ---- sums: to the slab in the order of the registers (16 bytes a lane, whole lines), or to their places
+  if (P.splits > 1) {
+f32x4* s = reinterpret_cast<f32x4*>(P.slab) + ((int64_t)(z * P.tiles + tile) * (TM * TN / 4)) + wave * (MI * NI * 4 * 64) + l;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f32x4 v;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] = acc[i][j][4 * e + c];
+          s[((i * NI + j) * 4 + e) * 64] = v;
+        }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int n = n0 + (wn * NI + j) * 32 + (l & 31);
+      if (n >= N) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int m = m0 + (wm * MI + i) * 32 + 8 * e + 4 * (l >> 5);
+        if (m >= M) continue;                             // (M is a multiple of 8)
+        float* o = P.out + (int64_t)m * N + n;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[(int64_t)c * N] = args.accumulate ? o[(int64_t)c * N] + acc[i][j][4 * e + c] : acc[i][j][4 * e + c];
+      }
+    }
+}
+
+// out (+)= the slabs of wgrad_bf16_kernel in the order of the row ranges; a block takes one (i, j) product of a wave: 256 f32x4 a slab
+template <int MI, int NI, int WM, int WN>
+__global__ __launch_bounds__(256) void wgrad_join_bf16_kernel(const Args args) {
+  constexpr int PER = WM * WN * MI * NI;                  // blocks a tile
+  const int l = threadIdx.x & 63, e = threadIdx.x >> 6;
+  int b = blockIdx.x, which = 0;
+  for (; which < args.count; ++which) {
+    const int mine = args.p[which].splits > 1 ? args.p[which].tiles * PER : 0;
+    if (b < mine) break;
+    b -= mine;
+  }
+  const Problem& P = args.p[which];
+  const int tile = b / PER, sub = b % PER, wave = sub / (MI * NI), ij = sub % (MI * NI);
+  const int n = tile % P.tiles_n * (32 * NI * WN) + (wave % WN * NI + ij % NI) * 32 + (l & 31);
+  const int m = tile / P.tiles_n * (32 * MI * WM) + (wave / WN * MI + ij / NI) * 32 + 8 * e + 4 * (l >> 5);
+  if (n >= P.N || m >= P.M) return;
+  const f32x4* s = reinterpret_cast<const f32x4*>(P.slab) + ((int64_t)tile * PER + sub) * 256 + threadIdx.x;
+  const int64_t stride = (int64_t)P.tiles * PER * 256;
+  f32x4 v = s[0];
+#pragma unroll 4
+  for (int z = 1; z < P.splits; ++z) v += s[z * stride];
+  float* o = P.out + (int64_t)m * P.N + n;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) o[(int64_t)c * P.N] = args.accumulate ? o[(int64_t)c * P.N] + v[c] : v[c];
+}
+
 // out (+)= the slabs in the order of the row ranges
 __global__ __launch_bounds__(256) void wgrad_join_kernel(const Args args) {
   for (int i = 0; i < args.count; ++i) {
@@ -141,33 +411,81 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const Args args) {
   }
 }
 
-// tiles and row ranges of the problems; returns the bytes of slabs, or -1
-int64_t plan(Args& a, int dtype) {
-  int64_t tiles = 0;
-  for (int i = 0; i < a.count; ++i) {
-    Problem& p = a.p[i];
-    if (p.M <= 0 || p.N <= 0 || p.rows <= 0 || p.M % 8 || p.N % ACTQ8_GROUP || p.rows > (1LL << 31) || (int64_t)p.M * p.N > (1LL << 31)) return -1;
-    p.tiles_n = ceil_div(p.N, BT);
-    p.tiles = ceil_div(p.M, BT) * p.tiles_n;
-    tiles += p.tiles;
-  }
+// Tile variants and the number of row ranges.  Time of a step of 64 rows with one tile on the chip's CUs or fewer (`one`) and with every
+// place taken (`full`: the clock drops with the power that the matrix units draw), measured on 2304 x 768 and 4096 x 4096; a range
+// costs about 3 us to start and end, a join 4 us and 5.5 TB/s for writing and reading the slabs.  The large tile moves the fewest
+// bytes per product, the small ones fill the chip on small outputs with fewer ranges, hence smaller slabs.
+struct Variant { int tm, tn, slots; double one, full; };
+constexpr Variant VAR[3] = {{256, 256, 256, 1.21, 1.65}, {256, 128, 256, 0.76, 0.97}, {128, 128, 512, 0.58, 1.11}};
+
+// sets tiles, row ranges and work of the problems for (tile, at most s ranges); returns the bytes of slabs
+int64_t lay_out(Args& a, int tm, int tn, int step, int s, bool exact_slabs) {
   int64_t bytes = 0, work = 0;
   for (int i = 0; i < a.count; ++i) {
     Problem& p = a.p[i];
-    p.steps = ceil_div(p.rows, BKR);
-    int64_t s = (512 + tiles / 2) / tiles;
-    if (s > p.steps / 8) s = p.steps / 8;
-    if (s < 1) s = 1;
-    p.steps_per_split = ceil_div(p.steps, s);
+    p.tiles_n = ceil_div(p.N, tn);
+    p.tiles = ceil_div(p.M, tm) * p.tiles_n;
+    p.steps = ceil_div(p.rows, step);
+    p.steps_per_split = ceil_div(p.steps, std::max(1, std::min(s, p.steps / 2)));
     p.splits = ceil_div(p.steps, p.steps_per_split);
     work += (int64_t)p.tiles * p.splits;
-    p.work_end = (int)work;
+    p.work_end = (int)std::min<int64_t>(work, INT32_MAX);
     if (p.splits > 1) {
       p.slab = reinterpret_cast<float*>(bytes);            // offset, resolved against the workspace by the caller
-      bytes += (int64_t)p.splits * p.M * p.N * 4;
+      bytes += (int64_t)p.splits * (exact_slabs ? (int64_t)p.M * p.N : (int64_t)p.tiles * tm * tn) * 4;
     }
   }
-  return work < (1LL << 31) ? bytes : -1;
+  return bytes;
+}
+
+// chooses the tile and the row ranges of the problems; returns the bytes of slabs, or -1
+int64_t plan(Args& a, int dtype) {
+  for (int i = 0; i < a.count; ++i) {
+    const Problem& p = a.p[i];
+    if (p.M <= 0 || p.N <= 0 || p.rows <= 0 || p.M % 8 || p.N % ACTQ8_GROUP || p.rows > (1LL << 31) || (int64_t)p.M * p.N > (1LL << 31)) return -1;
+  }
+  if (dtype == S4F_F32) {                                  // two tiles a CU, at least eight steps a range
+    lay_out(a, BT, BT, BKR, 1, true);
+    int steps = 0;
+    for (int i = 0; i < a.count; ++i) steps = std::max(steps, a.p[i].steps);
+    const int64_t bytes = lay_out(a, BT, BT, BKR, (int)std::max<int64_t>(1, std::min<int64_t>((512 + a.p[a.count - 1].work_end / 2) / a.p[a.count - 1].work_end, steps / 8)), true);
+    return a.p[a.count - 1].work_end < INT32_MAX ? bytes : -1;
+  }
+  double best = 0;
+  int bs = 0;
+  for (int v = 0; v < 3; ++v) {
+    int64_t tiles[MAXP], all = 0;
+    for (int i = 0; i < a.count; ++i) {
+      tiles[i] = (int64_t)ceil_div(a.p[i].M, VAR[v].tm) * ceil_div(a.p[i].N, VAR[v].tn);
+      all += tiles[i];
+    }
+    const int fill = (int)std::min<int64_t>(VAR[v].slots / all, 64);             // ranges that take every place once
+    for (int s : {1, 2, 3, 4, fill / 2, fill}) {
+      if (s < 1) continue;
+      int64_t items = 0, slabs = 0;
+      int longest = 0;
+      for (int i = 0; i < a.count; ++i) {
+        const int steps = ceil_div(a.p[i].rows, STEP), per = ceil_div(steps, std::max(1, std::min(s, steps / 2))), n = ceil_div(steps, per);
+        longest = std::max(longest, per);
+        items += tiles[i] * n;
+        if (n > 1) slabs += tiles[i] * n;
+      }
+      const double rest = (double)(items % VAR[v].slots) / VAR[v].slots, per = ((longest + 1) & ~1) + 0.25;
+      const double t = (double)(items / VAR[v].slots) * (per * VAR[v].full + 3) +
+                       (rest > 0 ? per * (VAR[v].one + rest * (VAR[v].full - VAR[v].one)) + 3 : 0) +
+                       (slabs ? 4 + 8e-6 / 5.5 * slabs * VAR[v].tm * VAR[v].tn : 0);
+      if (bs == 0 || t < best) { best = t; a.variant = v; bs = s; }
+    }
+  }
+  const int64_t bytes = lay_out(a, VAR[a.variant].tm, VAR[a.variant].tn, STEP, bs, false);
+  return a.p[a.count - 1].work_end < INT32_MAX ? bytes : -1;
+}
+
+template <int MI, int NI, int WM, int WN> void launch_bf16(const Args& a, hipStream_t st) {
+  hipLaunchKernelGGL((wgrad_bf16_kernel<MI, NI, WM, WN>), dim3(a.p[a.count - 1].work_end), dim3(64 * WM * WN), 0, st, a);
+  int blocks = 0;
+  for (int i = 0; i < a.count; ++i) blocks += a.p[i].splits > 1 ? a.p[i].tiles * WM * WN * MI * NI : 0;
+  if (blocks) hipLaunchKernelGGL((wgrad_join_bf16_kernel<MI, NI, WM, WN>), dim3(blocks), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -197,7 +515,7 @@ S4F_API int s4f_wgrad_packed(const s4f_wgrad_packed_desc* descs, int count, int 
     const s4f_wgrad_packed_desc& d = descs[i];
     S4F_CHECK(d.dy && d.codes && d.scales && d.out, "%s: null pointer in problem %d", who, i);
     S4F_CHECK((uintptr_t)d.dy % 16 == 0 && (uintptr_t)d.codes % 16 == 0 && (uintptr_t)d.out % 16 == 0 && d.lddy >= 0 &&
-                  d.lddy % (dtype == S4F_BF16 ? 8 : 4) == 0, "%s: rows of dy, codes and out must start on 16-byte boundaries (problem %d)", who, i);
+                  d.lddy % (dtype == S4F_BF16 ? 8 : 4) == 0 && d.lddy < (1 << 23), "%s: rows of dy, codes and out must start on 16-byte boundaries (problem %d)", who, i);
     S4F_CHECK(d.M > 0 && d.N > 0 && d.rows > 0 && d.M % 8 == 0 && d.N % ACTQ8_GROUP == 0,
               "%s: M=%d must be a multiple of 8, N=%d of 32, rows=%lld positive", who, d.M, d.N, (long long)d.rows);
     Problem& p = a.p[i];
@@ -215,9 +533,15 @@ S4F_API int s4f_wgrad_packed(const s4f_wgrad_packed_desc* descs, int count, int 
       join = true;
       n4 = std::max<int64_t>(n4, (int64_t)a.p[i].M * a.p[i].N / 4);
     }
+  if (dtype == S4F_BF16) {
+    if (a.variant == 0) launch_bf16<4, 2, 2, 4>(a, (hipStream_t)stream);
+    else if (a.variant == 1) launch_bf16<2, 2, 4, 2>(a, (hipStream_t)stream);
+    else launch_bf16<2, 2, 2, 2>(a, (hipStream_t)stream);
+    S4F_LAUNCH_CHECK();
+    return 0;
+  }
   const dim3 grid(a.p[count - 1].work_end);
-  if (dtype == S4F_BF16) hipLaunchKernelGGL(wgrad_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL(wgrad_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(wgrad_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, a);
   S4F_LAUNCH_CHECK();
   if (join) {
     hipLaunchKernelGGL(wgrad_join_kernel, dim3((unsigned)std::min<int64_t>((n4 + 255) / 256, 2048)), dim3(256), 0, (hipStream_t)stream, a);

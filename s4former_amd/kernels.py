@@ -509,37 +509,40 @@ def attention_bwd_fused(qkv, ctx, dctx, lse, delta, dqkv, B, N, H, ws, bias_u=No
 
 
 # ------------------------------------------------------------------------------------------------ norm + rotation of queries and keys
-def _here(t):
-    return t.is_cuda and t.get_device() == L._cur_device()
+# The operators below are also called at sizes where the launch is all there is, so their checks read each attribute of a tensor once.
+def _dev(t):
+    """the current device's index if t is a device tensor, else an index that no tensor has"""
+    return L._cur_device() if t.is_cuda else -2
 
 
-def _mat(t, dtype, cols, what):
-    """[rows, cols] device matrix, possibly a column slice of a wider buffer -> (pointer, row stride in elements).  A single row has
-    no stride worth the name (torch may report any)."""
-    if t.dim() != 2 or t.shape[1] != cols or t.dtype != dtype:
-        raise S4FError(f'{what}: expected a [rows, {cols}] {dtype} matrix, got {tuple(t.shape)} {t.dtype}')
-    if not _here(t):
+def _mat(t, dtype, cols, dev, what):
+    """[rows, cols] matrix on device dev, possibly a column slice of a wider buffer -> (pointer, row stride in elements, rows).  A single
+    row has no stride worth the name (torch may report any)."""
+    sh = t.shape
+    if len(sh) != 2 or sh[1] != cols or t.dtype is not dtype:
+        raise S4FError(f'{what}: expected a [rows, {cols}] {dtype} matrix, got {tuple(sh)} {t.dtype}')
+    if t.get_device() != dev:
         raise S4FError(f'{what}: expected a tensor on the current device')
-    if cols > 1 and t.stride(1) != 1:
+    ld, one = t.stride()
+    if one != 1 and cols > 1:
         raise S4FError(f'{what}: the elements of a row must be contiguous')
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else cols
+    rows = sh[0]
+    return t.data_ptr(), ld if rows > 1 else cols, rows
 
 
-def _vec(t, dtype, n, what):
-    """contiguous device tensor of n elements -> pointer (None -> NULL)"""
-    if t is None:
-        return None
-    if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or not _here(t):
+def _vec(t, dtype, n, dev, what):
+    """contiguous tensor of n elements on device dev -> pointer"""
+    if t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
         raise S4FError(f'{what}: expected a contiguous {dtype} tensor of {n} elements on the current device, got {tuple(t.shape)} {t.dtype}')
     return t.data_ptr()
 
 
-def _buf(t, need, what):
-    """workspace of at least `need` bytes -> (pointer, bytes)"""
-    if need == 0:
+def _buf(t, dev, what):
+    """workspace -> (pointer, bytes); the entry point compares its size with the need"""
+    if t is None:
         return None, 0
-    if t is None or not t.is_contiguous() or not _here(t) or t.numel() * t.element_size() < need:
-        raise S4FError(f'{what}: expected a contiguous workspace of at least {need} bytes on the current device')
+    if t.get_device() != dev or not t.is_contiguous():
+        raise S4FError(f'{what}: expected a contiguous workspace on the current device')
     return t.data_ptr(), t.numel() * t.element_size()
 
 
@@ -555,26 +558,41 @@ def _apart(pa, lda, pb, ldb, rows, row_bytes, es, what):
     raise S4FError(f'{what} overlap')
 
 
-def _qk_common(x, rows, heads, gq, gk, cos, sin, what):
+def _launch(name, *args):
+    if L._prof is not None or L._lib is None:
+        return call(name, *args)
+    if getattr(L._lib, name)(*args):
+        raise S4FError(f'{name} failed: {L._lib.s4f_last_error().decode(errors="replace")}')
+
+
+def _stream_of(dev):
+    return L._raw_stream(dev) if L._raw_stream is not None else stream()
+
+
+def _gains_tables(rows, gq, gk, cos, sin, dev, what):
+    """pointers of the gains and tables (None -> NULL) and the number of positions"""
     if (gq is None) != (gk is None) or (cos is None) != (sin is None):
         raise S4FError(f'{what}: gains (gq, gk) and tables (cos, sin) come in pairs')
-    if gq is None and cos is None:
+    f32 = torch.float32
+    if gq is not None:
+        gq, gk = _vec(gq, f32, 64, dev, what + ' gq'), _vec(gk, f32, 64, dev, what + ' gk')
+    elif cos is None:
         raise S4FError(f'{what}: neither a norm (gq, gk) nor a rotation (cos, sin) asked for')
     period = 0
     if cos is not None:
-        if cos.dim() != 2 or cos.shape[1] != 32 or cos.shape != sin.shape:
+        sh = cos.shape
+        if len(sh) != 2 or sh[1] != 32:
             raise S4FError(f'{what}: cos and sin must be [positions, 32]')
-        period = cos.shape[0]
+        period = sh[0]
         if period == 0 or rows % period:
             raise S4FError(f'{what}: {period} positions do not divide {rows} rows')
-    f32 = torch.float32
-    return (_vec(gq, f32, 64, what + ' gq'), _vec(gk, f32, 64, what + ' gk'), _vec(cos, f32, period * 32, what + ' cos'),
-            _vec(sin, f32, period * 32, what + ' sin'), period)
+        cos, sin = _vec(cos, f32, period * 32, dev, what + ' cos'), _vec(sin, f32, period * 32, dev, what + ' sin')
+    return gq, gk, cos, sin, period
 
 
-def _packed_ptrs(packed, rows, C, what):
+def _packed_ptrs(packed, rows, C, dev, what):
     codes, scales = packed
-    return _vec(codes, torch.int8, rows * C, what + ' codes'), _vec(scales, torch.uint8, rows * (C // 32), what + ' scales')
+    return _vec(codes, torch.int8, rows * C, dev, what + ' codes'), _vec(scales, torch.uint8, rows * (C // 32), dev, what + ' scales')
 
 
 def qk_norm_rope_fwd(x, y, Hq, Hk, dtype, gq=None, gk=None, cos=None, sin=None, eps=1e-6, packed=None):
@@ -582,20 +600,22 @@ def qk_norm_rope_fwd(x, y, Hq, Hk, dtype, gq=None, gk=None, cos=None, sin=None, 
     angles of their rows (cos, sin [positions, 32], if given; row r has position r % positions).  x and y may be column slices of
     wider buffers, and the same one.  packed: (codes int8 [rows, (Hq + Hk) 64], scales uint8 [rows, (Hq + Hk) 2]) receive the 8-bit
     checkpoint of the pre-norm x that qk_norm_rope_bwd reads."""
-    C, rows, T = (Hq + Hk) * 64, x.shape[0], _tdt(dtype)
-    xp, ldx = _mat(x, T, C, 'qk_norm_rope_fwd x')
-    yp, ldy = _mat(y, T, C, 'qk_norm_rope_fwd y')
-    if y.shape[0] != rows:
-        raise S4FError(f'qk_norm_rope_fwd: x has {rows} rows, y {y.shape[0]}')
-    if packed is not None and gq is None:
-        raise S4FError('qk_norm_rope_fwd: the rotation alone needs no checkpoint')
+    C, T, dev = (Hq + Hk) * 64, _tdt(dtype), _dev(x)
+    xp, ldx, rows = _mat(x, T, C, dev, 'qk_norm_rope_fwd x')
+    yp, ldy, yrows = _mat(y, T, C, dev, 'qk_norm_rope_fwd y')
+    if yrows != rows:
+        raise S4FError(f'qk_norm_rope_fwd: x has {rows} rows, y {yrows}')
+    codes = scales = None
+    if packed is not None:
+        if gq is None:
+            raise S4FError('qk_norm_rope_fwd: the rotation alone needs no checkpoint')
+        codes, scales = _packed_ptrs(packed, rows, C, dev, 'qk_norm_rope_fwd')
     if rows == 0:
         return
-    gqp, gkp, cp, sp, period = _qk_common(x, rows, Hq + Hk, gq, gk, cos, sin, 'qk_norm_rope_fwd')
-    codes, scales = _packed_ptrs(packed, rows, C, 'qk_norm_rope_fwd') if packed is not None else (None, None)
-    es = x.element_size()
+    gq, gk, cos, sin, period = _gains_tables(rows, gq, gk, cos, sin, dev, 'qk_norm_rope_fwd')
+    es = 2 if dtype == BF16 else 4
     _apart(xp, ldx, yp, ldy, rows, C * es, es, 'qk_norm_rope_fwd: x and y')
-    call('s4f_qk_norm_rope_fwd', xp, ldx, yp, ldy, gqp, gkp, cp, sp, period, eps, codes, scales, rows, Hq, Hk, dtype, stream())
+    _launch('s4f_qk_norm_rope_fwd', xp, ldx, yp, ldy, gq, gk, cos, sin, period, eps, codes, scales, rows, Hq, Hk, dtype, _stream_of(dev))
 
 
 def qk_norm_rope_ws_bytes(rows, Hq, Hk):
@@ -606,36 +626,37 @@ def qk_norm_rope_bwd(dy, dx, Hq, Hk, dtype, x=None, packed=None, gq=None, gk=Non
                      ws=None, accumulate=True):
     """Backward of qk_norm_rope_fwd: dx from dy (dx may be dy) and, with the norm, the pre-norm x or its checkpoint `packed`; the
     gain gradients are added to dgq / dgk fp32 [64] (accumulate=False: written).  ws: qk_norm_rope_ws_bytes(rows, Hq, Hk) bytes."""
-    C, rows, T = (Hq + Hk) * 64, dy.shape[0], _tdt(dtype)
-    dyp, lddy = _mat(dy, T, C, 'qk_norm_rope_bwd dy')
-    dxp, lddx = _mat(dx, T, C, 'qk_norm_rope_bwd dx')
-    if dx.shape[0] != rows:
-        raise S4FError(f'qk_norm_rope_bwd: dy has {rows} rows, dx {dx.shape[0]}')
-    if gq is not None and ((x is None) == (packed is None) or dgq is None or dgk is None):
-        raise S4FError('qk_norm_rope_bwd: the norm needs x or packed (not both), dgq and dgk')
-    f32 = torch.float32
-    dgqp, dgkp = (_vec(dgq, f32, 64, 'qk_norm_rope_bwd dgq'), _vec(dgk, f32, 64, 'qk_norm_rope_bwd dgk')) if gq is not None else (None, None)
-    if dgqp is not None and dgqp == dgkp:
-        raise S4FError('qk_norm_rope_bwd: dgq and dgk overlap')
+    C, T, dev, norm = (Hq + Hk) * 64, _tdt(dtype), _dev(dy), gq is not None
+    dyp, lddy, rows = _mat(dy, T, C, dev, 'qk_norm_rope_bwd dy')
+    dxp, lddx, xrows = _mat(dx, T, C, dev, 'qk_norm_rope_bwd dx')
+    if xrows != rows:
+        raise S4FError(f'qk_norm_rope_bwd: dy has {rows} rows, dx {xrows}')
+    es = 2 if dtype == BF16 else 4
+    xp = codes = scales = wsp = dgqp = dgkp = None
+    ldx = wsb = 0
+    if norm:
+        if (x is None) == (packed is None) or dgq is None or dgk is None:
+            raise S4FError('qk_norm_rope_bwd: the norm needs x or packed (not both), dgq and dgk')
+        dgqp, dgkp = _vec(dgq, torch.float32, 64, dev, 'qk_norm_rope_bwd dgq'), _vec(dgk, torch.float32, 64, dev, 'qk_norm_rope_bwd dgk')
+        if abs(dgqp - dgkp) < 256:
+            raise S4FError('qk_norm_rope_bwd: dgq and dgk overlap')
+        if packed is not None:
+            codes, scales = _packed_ptrs(packed, rows, C, dev, 'qk_norm_rope_bwd')
+        else:
+            xp, ldx, xrows = _mat(x, T, C, dev, 'qk_norm_rope_bwd x')
+            if xrows != rows:
+                raise S4FError(f'qk_norm_rope_bwd: dy has {rows} rows, x {xrows}')
+            if rows:
+                _apart(xp, ldx, dxp, lddx, rows, C * es, es, 'qk_norm_rope_bwd: x and dx')
+        wsp, wsb = _buf(ws, dev, 'qk_norm_rope_bwd ws')
     if rows == 0:
-        if gq is not None and not accumulate:
+        if norm and not accumulate:
             dgq.zero_(); dgk.zero_()
         return
-    gqp, gkp, cp, sp, period = _qk_common(dy, rows, Hq + Hk, gq, gk, cos, sin, 'qk_norm_rope_bwd')
-    es = dy.element_size()
+    gq, gk, cos, sin, period = _gains_tables(rows, gq, gk, cos, sin, dev, 'qk_norm_rope_bwd')
     _apart(dyp, lddy, dxp, lddx, rows, C * es, es, 'qk_norm_rope_bwd: dy and dx')
-    xp, ldx, codes, scales, wsp, wsb = None, 0, None, None, None, 0
-    if gq is not None:
-        if packed is not None:
-            codes, scales = _packed_ptrs(packed, rows, C, 'qk_norm_rope_bwd')
-        else:
-            xp, ldx = _mat(x, T, C, 'qk_norm_rope_bwd x')
-            if x.shape[0] != rows:
-                raise S4FError(f'qk_norm_rope_bwd: dy has {rows} rows, x {x.shape[0]}')
-            _apart(xp, ldx, dxp, lddx, rows, C * es, es, 'qk_norm_rope_bwd: x and dx')
-        wsp, wsb = _buf(ws, qk_norm_rope_ws_bytes(rows, Hq, Hk), 'qk_norm_rope_bwd ws')
-    call('s4f_qk_norm_rope_bwd', dyp, lddy, xp, ldx, codes, scales, dxp, lddx, gqp, gkp, cp, sp, period, eps, dgqp, dgkp,
-         1 if accumulate else 0, wsp, wsb, rows, Hq, Hk, dtype, stream())
+    _launch('s4f_qk_norm_rope_bwd', dyp, lddy, xp, ldx, codes, scales, dxp, lddx, gq, gk, cos, sin, period, eps, dgqp, dgkp,
+            1 if accumulate else 0, wsp, wsb, rows, Hq, Hk, dtype, _stream_of(dev))
 
 
 # ------------------------------------------------------------------------------------------------ activation checkpoints in 8 bits
@@ -646,26 +667,23 @@ def _group_cols(C, what):
 
 def act_pack(x, codes, scales, dtype):
     """8-bit checkpoint of x [rows, C] (C a multiple of 32; a column slice of a wider buffer qualifies): codes int8 [rows, C], scales uint8
-    [rows, C / 32].  |x - restored| <= max |x| / 127.5 over the 32 channels; a group with an infinity or a NaN comes
-    back as NaN."""
-    C = x.shape[-1]
+    [rows, C / 32].  |x - restored| <= max |x| / 127.5 over the 32 channels; a group with an infinity or a NaN comes back as NaN."""
+    C, dev = x.shape[-1], _dev(x)
     _group_cols(C, 'act_pack')
-    xp, ldx = _mat(x, _tdt(dtype), C, 'act_pack x')
-    rows = x.shape[0]
-    cp, sp = _packed_ptrs((codes, scales), rows, C, 'act_pack')
+    xp, ldx, rows = _mat(x, _tdt(dtype), C, dev, 'act_pack x')
+    codes, scales = _packed_ptrs((codes, scales), rows, C, dev, 'act_pack')
     if rows:
-        call('s4f_act_pack', xp, ldx, cp, sp, rows, C, dtype, stream())
+        _launch('s4f_act_pack', xp, ldx, codes, scales, rows, C, dtype, _stream_of(dev))
 
 
 def act_unpack(codes, scales, y, dtype):
     """y [rows, C] = the activation that act_pack put away"""
-    C = y.shape[-1]
+    C, dev = y.shape[-1], _dev(y)
     _group_cols(C, 'act_unpack')
-    yp, ldy = _mat(y, _tdt(dtype), C, 'act_unpack y')
-    rows = y.shape[0]
-    cp, sp = _packed_ptrs((codes, scales), rows, C, 'act_unpack')
+    yp, ldy, rows = _mat(y, _tdt(dtype), C, dev, 'act_unpack y')
+    codes, scales = _packed_ptrs((codes, scales), rows, C, dev, 'act_unpack')
     if rows:
-        call('s4f_act_unpack', cp, sp, yp, ldy, rows, C, dtype, stream())
+        _launch('s4f_act_unpack', codes, scales, yp, ldy, rows, C, dtype, _stream_of(dev))
 
 
 def wgrad_packed_ws_bytes(problems, dtype):
@@ -679,20 +697,21 @@ def wgrad_packed(problems, dtype, ws=None, accumulate=True):
     one where the rows are split.  ws: wgrad_packed_ws_bytes([(M, N, rows), ...], dtype) bytes."""
     if not 1 <= len(problems) <= 4:
         raise S4FError('wgrad_packed: 1..4 problems')
-    T = _tdt(dtype)
-    descs, dims, spans = [], [], []
+    T, dev = _tdt(dtype), _dev(problems[0][3])
+    descs, spans = [], []
     for dy, codes, scales, out in problems:
-        if out.dim() != 2 or out.shape[0] % 8 or out.shape[1] % 32 or out.shape[0] == 0 or out.shape[1] == 0:
-            raise S4FError(f'wgrad_packed: out must be [M, N] with M a multiple of 8 and N of 32, got {tuple(out.shape)}')
-        M, N = out.shape
-        dyp, ld = _mat(dy, T, M, 'wgrad_packed dy')
-        rows = dy.shape[0]
-        cp, sp = _packed_ptrs((codes, scales), rows, N, 'wgrad_packed')
-        op = _vec(out, torch.float32, M * N, 'wgrad_packed out')
+        sh = out.shape
+        if len(sh) != 2 or sh[0] % 8 or sh[1] % 32 or sh[0] == 0 or sh[1] == 0:
+            raise S4FError(f'wgrad_packed: out must be [M, N] with M a multiple of 8 and N of 32, got {tuple(sh)}')
+        M, N = sh
+        dyp, ld, rows = _mat(dy, T, M, dev, 'wgrad_packed dy')
+        if ld < M:
+            raise S4FError('wgrad_packed dy: the rows overlap')
+        cp, sp = _packed_ptrs((codes, scales), rows, N, dev, 'wgrad_packed')
+        op = _vec(out, torch.float32, M * N, dev, 'wgrad_packed out')
         spans.append((op, op + 4 * M * N))
         if rows:
             descs.append((dyp, ld, cp, sp, op, rows, M, N))
-            dims += [M, N, rows]
         elif not accumulate:
             out.zero_()
     if len(spans) > 1:
@@ -701,9 +720,9 @@ def wgrad_packed(problems, dtype, ws=None, accumulate=True):
             raise S4FError('wgrad_packed: the outputs overlap')
     if not descs:
         return
-    wsp, wsb = _buf(ws, workspace_bytes(WS_WGRAD_PACKED, dtype, *dims), 'wgrad_packed ws')
+    wsp, wsb = _buf(ws, dev, 'wgrad_packed ws')
     arr = (L.WgradPackedDesc * len(descs))(*descs)
-    call('s4f_wgrad_packed', arr, len(descs), dtype, 1 if accumulate else 0, wsp, wsb, stream())
+    _launch('s4f_wgrad_packed', arr, len(descs), dtype, 1 if accumulate else 0, wsp, wsb, _stream_of(dev))
 
 
 def bn_stats(x, rows, C, sums, dtype):
