@@ -13,6 +13,7 @@
 // the heads of a row being neighbours in the grid.
 #include "actq8.h"
 #include "../../include/s4f.h"
+#include <algorithm>
 
 namespace {
 
@@ -47,6 +48,7 @@ template <typename T> __device__ __forceinline__ chunk16 pack16(const float (&v)
   for (int i = 0; i < (int)(16 / sizeof(T)); ++i) u.t[i] = from_f32<T>(v[i]);
   return u.c;
 }
+template <int V> struct __attribute__((aligned(V))) Codes { uint32_t w[V / 4]; };           // V codes of a lane
 template <int V> __device__ __forceinline__ void ld_f32(const float* p, float (&v)[V]) {
 #pragma unroll
   for (int i = 0; i < V; i += 4) {
@@ -83,14 +85,14 @@ __global__ __launch_bounds__(256) void qk_fwd_kernel(const QkArgs a) {
     const uint32_t bl = q8_scale_byte(group_max<LANES>(ml)), bh = q8_scale_byte(group_max<LANES>(mh));
     const float il = q8_inv_scale(bl), ih = q8_inv_scale(bh);
     int8_t* cp = a.codes + ((int64_t)row * a.H + h) * 64 + l * V;
+    Codes<V> wl, wh;
 #pragma unroll
-    for (int e = 0; e < V; e += 4) {
-      uint32_t wl = q8_codes4(lo[e], lo[e + 1], lo[e + 2], lo[e + 3], il), wh = q8_codes4(hi[e], hi[e + 1], hi[e + 2], hi[e + 3], ih);
-      if (bl == 255u) wl = 0;
-      if (bh == 255u) wh = 0;
-      *reinterpret_cast<uint32_t*>(cp + e) = wl;
-      *reinterpret_cast<uint32_t*>(cp + 32 + e) = wh;
+    for (int e = 0; e < V / 4; ++e) {
+      wl.w[e] = bl == 255u ? 0u : q8_codes4(lo[4 * e], lo[4 * e + 1], lo[4 * e + 2], lo[4 * e + 3], il);
+      wh.w[e] = bh == 255u ? 0u : q8_codes4(hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3], ih);
     }
+    *reinterpret_cast<Codes<V>*>(cp) = wl;
+    *reinterpret_cast<Codes<V>*>(cp + 32) = wh;
     if (l == 0) *reinterpret_cast<uint16_t*>(a.scales + ((int64_t)row * a.H + h) * 2) = (uint16_t)(bl | (bh << 8));
   }
   if constexpr (NORM) {
@@ -155,12 +157,9 @@ __global__ __launch_bounds__(256) void qk_bwd_kernel(const QkArgs a) {
       const int8_t* cp = a.codes + hd * 64 + l * V;
       const uint32_t by = *reinterpret_cast<const uint16_t*>(a.scales + hd * 2);
       const float sl = q8_scale(by & 255u), sh = q8_scale(by >> 8);
+      const Codes<V> wl = *reinterpret_cast<const Codes<V>*>(cp), wh = *reinterpret_cast<const Codes<V>*>(cp + 32);
 #pragma unroll
-      for (int e = 0; e < V; e += 4) {
-        const uint32_t wl = *reinterpret_cast<const uint32_t*>(cp + e), wh = *reinterpret_cast<const uint32_t*>(cp + 32 + e);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) { xl[e + k] = q8_code(wl, k) * sl; xh[e + k] = q8_code(wh, k) * sh; }
-      }
+      for (int e = 0; e < V; ++e) { xl[e] = q8_code(wl.w[e / 4], e & 3) * sl; xh[e] = q8_code(wh.w[e / 4], e & 3) * sh; }
     }
     unpack16<T>(d0, lo);
     unpack16<T>(d1, hi);
@@ -219,30 +218,33 @@ __global__ __launch_bounds__(256) void qk_bwd_kernel(const QkArgs a) {
   }
 }
 
-// gain gradients from the blocks' partial sums: block = (kind, 16 of the 64 channels), 16 threads a channel
+// gain gradients from the blocks' partial sums: block = (kind, four of the 64 channels), its threads over the partial sums
 __global__ __launch_bounds__(256) void qk_gain_kernel(const float* __restrict__ part, int bq, int blocks, float* __restrict__ dgq,
                                                       float* __restrict__ dgk, int accumulate) {
-  __shared__ float sum[16][17];
-  const bool key = blockIdx.x >= 4;
-  const int c = (blockIdx.x & 3) * 16 + (threadIdx.x & 15), t = threadIdx.x >> 4;
-  const int end = key ? blocks : bq;
-  float s = 0.f;
-#pragma unroll 8
-  for (int b = (key ? bq : 0) + t; b < end; b += 16) s += part[(int64_t)b * 64 + c];
-  sum[t][threadIdx.x & 15] = s;
+  __shared__ f32x4 sum[4];
+  const bool key = blockIdx.x >= 16;
+  const int c = (blockIdx.x & 15) * 4, end = key ? blocks : bq;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int b = (key ? bq : 0) + threadIdx.x; b < end; b += 256) s += *reinterpret_cast<const f32x4*>(part + (int64_t)b * 64 + c);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s[e] = wave_sum(s[e]);
+  if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x < 16) {
-    float v = 0.f;
-    for (int i = 0; i < 16; ++i) v += sum[i][threadIdx.x];
-    float* o = (key ? dgk : dgq) + c;
+  if (threadIdx.x < 4) {
+    const int e = threadIdx.x;
+    const float v = (sum[0][e] + sum[1][e]) + (sum[2][e] + sum[3][e]);
+    float* o = (key ? dgk : dgq) + c + e;
     *o = accumulate ? *o + v : v;
   }
 }
 
-// blocks of the backward for n heads of one kind: eight per CU at most (256 CUs), each with at least one full turn of its lanes
-int bwd_blocks(int64_t items, int per) {
-  const int64_t b = (items + per - 1) / per;
-  return (int)(b < 1024 ? b : 1024);
+// blocks of the backward for the heads of one kind: 1,024 in all at most, in proportion, each with at least one full turn of its lanes.
+// (Measured at 16,400 rows x 24 heads, bf16: 512 a kind 25.8 us, 384 26.3, 1,024 26.8, 2,048 30.2: the blocks end with a reduction and
+// leave 256 bytes each to be joined.)
+int bwd_blocks(int64_t rows, int heads, int all, int per) {
+  const int64_t b = (rows * heads + per - 1) / per, cap = std::max(1, 1024 * heads / all);
+  return (int)std::min(b, cap);
 }
 
 int check_qk(const char* who, int64_t rows, int Hq, int Hk, int dtype, const float* gq, const float* gk, const float* cos,
@@ -306,7 +308,7 @@ S4F_API int s4f_qk_norm_rope_fwd(const void* x, int64_t ldx, void* y, int64_t ld
 
 int64_t s4f_qk_ws_bytes(int64_t rows, int Hq, int Hk) {
   if (rows <= 0 || Hq <= 0 || Hk <= 0) return -1;
-  return ((int64_t)bwd_blocks(rows * Hq, 32) + bwd_blocks(rows * Hk, 32)) * 64 * 4;
+  return ((int64_t)bwd_blocks(rows, Hq, Hq + Hk, 32) + bwd_blocks(rows, Hk, Hq + Hk, 32)) * 64 * 4;
 }
 
 S4F_API int s4f_qk_norm_rope_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int8_t* codes, const uint8_t* scales,
@@ -332,12 +334,12 @@ S4F_API int s4f_qk_norm_rope_bwd(const void* dy, int64_t lddy, const void* x, in
   a.codes = gq ? const_cast<int8_t*>(codes) : nullptr; a.scales = const_cast<uint8_t*>(scales); a.part = (float*)ws; a.eps = eps;
   a.rows = (uint32_t)rows; a.period = (uint32_t)(cos ? period : 1); a.Hq = Hq; a.H = Hq + Hk;
   const int per = dtype == S4F_BF16 ? 64 : 32;
-  a.bq = bwd_blocks(rows * Hq, per);
-  const int blocks = a.bq + bwd_blocks(rows * Hk, per);
+  a.bq = bwd_blocks(rows, Hq, Hq + Hk, per);
+  const int blocks = a.bq + bwd_blocks(rows, Hk, Hq + Hk, per);
   if (dtype == S4F_BF16) launch_bwd<bf16_t>(a, blocks, (hipStream_t)stream); else launch_bwd<float>(a, blocks, (hipStream_t)stream);
   S4F_LAUNCH_CHECK();
   if (gq) {
-    hipLaunchKernelGGL(qk_gain_kernel, dim3(8), dim3(256), 0, (hipStream_t)stream, (const float*)ws, a.bq, blocks, dgq, dgk, accumulate);
+    hipLaunchKernelGGL(qk_gain_kernel, dim3(32), dim3(256), 0, (hipStream_t)stream, (const float*)ws, a.bq, blocks, dgq, dgk, accumulate);
     S4F_LAUNCH_CHECK();
   }
   return 0;

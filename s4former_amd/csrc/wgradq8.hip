@@ -26,17 +26,13 @@ struct Problem {
 };
 struct Args { Problem p[MAXP]; int count, accumulate, variant; };
 
-// ------------------------------------------------------------------------------------------------- 128 x 128 tile, any type
-constexpr int BT = 128, BKR = 32;
-template <typename T> constexpr int lds_stride() { return BT * (int)sizeof(T) + 16; }
+// ------------------------------------------------------------------------------------------------- fp32
+// 64 x 64 tile, four waves of 32 x 32, 32 rows a step, two buffers; several tiles a CU hide the latency of loads and reads.  The fp32
+// matrix rate (256 operations a clock and CU) bounds large problems; the small tile keeps ragged sizes from wasting it.
+constexpr int BT = 64, BKR = 32, LDF = BT * 4 + 16;      // bytes of a row in LDS: rows 4 apart lie 16 banks apart
 
-template <typename T>
-__global__ __launch_bounds__(256) void wgrad_kernel(const Args args) {
-  constexpr int V = 16 / sizeof(T), NA = BKR * (BT / V) / 256, LD = lds_stride<T>();
-  __shared__ __attribute__((aligned(16))) char smem[2 * BKR * LD];
-  char* const la = smem;
-  char* const lb = smem + BKR * LD;
-
+__global__ __launch_bounds__(256) void wgrad_f32_kernel(const Args args) {
+  __shared__ __attribute__((aligned(16))) char la[2][BKR * LDF], lb[2][BKR * LDF];
   int which = 0;
   for (int i = 0; i < MAXP - 1; ++i) which += i < args.count - 1 && (int)blockIdx.x >= args.p[i].work_end ? 1 : 0;
   const Problem& P = args.p[which];
@@ -44,77 +40,70 @@ __global__ __launch_bounds__(256) void wgrad_kernel(const Args args) {
   const int z = local / P.tiles, tile = local - z * P.tiles;
   const int m0 = tile / P.tiles_n * BT, n0 = tile % P.tiles_n * BT;
   const int k_beg = z * P.steps_per_split, k_end = min(k_beg + P.steps_per_split, P.steps);
-
-  const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, g = l >> 4, li = l & 15;
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  const T* dy = reinterpret_cast<const T*>(P.dy);
   const int N = P.N, M = P.M;
 
-  chunk16 ra[NA], rb;
-  uint32_t rs;
-  auto load = [&](int k) {
-    const int64_t r0 = (int64_t)k * BKR;
+  const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, g = l >> 4, li = l & 15;
+  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
+  // a thread's chunks: rows tid / 16 and + 16 of dY, four values; row tid / 8 of the codes, eight values (M is a multiple of 8 and N of
+  // 32: a chunk is inside or outside)
+  const int ra = tid >> 4, ca = (tid & 15) * 4, rb = tid >> 3, cb = (tid & 7) * 8;
+  const bool aok = m0 + ca < M, bok = n0 + cb < N;
+  const float* pa = reinterpret_cast<const float*>(P.dy) + ((int64_t)k_beg * BKR + ra) * P.lddy + m0 + ca;
+  const int8_t* pb = P.codes + ((int64_t)k_beg * BKR + rb) * N + n0 + cb;
+  const uint8_t* ps = P.scales + ((int64_t)k_beg * BKR + rb) * (N / ACTQ8_GROUP) + (n0 + cb) / ACTQ8_GROUP;
+  int64_t left = P.rows - (int64_t)k_beg * BKR;            // rows from the step on
+
+  chunk16 xa[2];
+  uint2 xb;
+  uint32_t xs;
+  auto load = [&]() {
 #pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      const int c = tid + i * 256, row = c / (BT / V), col = (c % (BT / V)) * V;
-      const bool ok = r0 + row < P.rows && m0 + col < M;     // (M is a multiple of 8: a chunk is inside or outside)
-      ra[i] = ok ? ld_global16(dy + (r0 + row) * P.lddy + m0 + col) : zero16();
-    }
-    const int row = tid >> 3, col = (tid & 7) * 16;
-    const bool ok = r0 + row < P.rows && n0 + col < N;
-    rb = ok ? ld_global16(P.codes + (r0 + row) * N + n0 + col) : zero16();
-    rs = ok ? P.scales[(r0 + row) * (N / ACTQ8_GROUP) + (n0 + col) / ACTQ8_GROUP] : 0u;
+    for (int i = 0; i < 2; ++i) xa[i] = aok && ra + 16 * i < left ? ld_global16(pa + (int64_t)(16 * i) * P.lddy) : zero16();
+    const bool ok = bok && rb < left;
+    xb = ok ? *reinterpret_cast<const uint2*>(pb) : make_uint2(0, 0);
+    xs = ok ? *ps : 0u;
+    pa += (int64_t)BKR * P.lddy; pb += (int64_t)BKR * N; ps += (int64_t)BKR * (N / ACTQ8_GROUP); left -= BKR;
   };
-  auto store = [&]() {
+  auto store = [&](int buf) {
 #pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      const int c = tid + i * 256, row = c / (BT / V), col = (c % (BT / V)) * V;
-      *reinterpret_cast<chunk16*>(la + row * LD + col * (int)sizeof(T)) = ra[i];
-    }
-    const float s = q8_scale(rs);
-    char* o = lb + (tid >> 3) * LD + (tid & 7) * 16 * (int)sizeof(T);
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<chunk16*>(la[buf] + (ra + 16 * i) * LDF + ca * 4) = xa[i];
+    const float s = q8_scale(xs);
+    f32x4 v0, v1;
 #pragma unroll
-    for (int i = 0; i < 16; i += V) {
-      chunk16 c;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (V == 8) c.w[e] = pack_exact_bf16(q8_code(rb.w[(i + 2 * e) / 4], (2 * e) & 3) * s, q8_code(rb.w[(i + 2 * e) / 4], (2 * e + 1) & 3) * s);
-        else c.w[e] = __float_as_uint(q8_code(rb.w[i / 4], e) * s);
-      }
-      *reinterpret_cast<chunk16*>(o + i * (int)sizeof(T)) = c;
-    }
+    for (int e = 0; e < 4; ++e) { v0[e] = q8_code(xb.x, e) * s; v1[e] = q8_code(xb.y, e) * s; }
+    *reinterpret_cast<f32x4*>(lb[buf] + rb * LDF + cb * 4) = v0;
+    *reinterpret_cast<f32x4*>(lb[buf] + rb * LDF + cb * 4 + 16) = v1;
   };
 
-  f32x4 acc[4][4];
+  f32x4 acc[2][2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  if (k_beg < k_end) load(k_beg);
+    for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (k_beg < k_end) { load(); store(0); }
   for (int k = k_beg; k < k_end; ++k) {
+    const int buf = (k - k_beg) & 1;
+    if (k + 1 < k_end) load();
     __syncthreads();
-    store();
-    __syncthreads();
-    if (k + 1 < k_end) load(k + 1);
-    Frag<T> b[4];
+    Frag<float> a[2], b[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) lds_read_tr(b[j], lb, LD, 0, wn + j * 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      Frag<T> a;
-      lds_read_tr(a, la, LD, 0, wm + i * 16);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mma16(a, b[j], acc[i][j]);
+    for (int i = 0; i < 2; ++i) {
+      lds_read_tr(a[i], la[buf], LDF, 0, wm + i * 16);
+      lds_read_tr(b[i], lb[buf], LDF, 0, wn + i * 16);
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j] = mma16(a[i], b[j], acc[i][j]);
+    if (k + 1 < k_end) store(buf ^ 1);                     // (last read in the step before: everyone has passed the barrier since)
   }
 
   const bool add = P.splits == 1 && args.accumulate;
   float* o = P.splits == 1 ? P.out : P.slab + (int64_t)z * M * N;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
       const int n = n0 + wn + j * 16 + li;
       if (n >= N) continue;
 #pragma unroll
@@ -397,7 +386,7 @@ __global__ __launch_bounds__(256) void wgrad_join_bf16_kernel(const Args args) {
   for (int c = 0; c < 4; ++c) o[(int64_t)c * P.N] = args.accumulate ? o[(int64_t)c * P.N] + v[c] : v[c];
 }
 
-// out (+)= the slabs in the order of the row ranges
+// out (+)= the slabs of wgrad_f32_kernel in the order of the row ranges
 __global__ __launch_bounds__(256) void wgrad_join_kernel(const Args args) {
   for (int i = 0; i < args.count; ++i) {
     const Problem& P = args.p[i];
@@ -444,11 +433,12 @@ int64_t plan(Args& a, int dtype) {
     const Problem& p = a.p[i];
     if (p.M <= 0 || p.N <= 0 || p.rows <= 0 || p.M % 8 || p.N % ACTQ8_GROUP || p.rows > (1LL << 31) || (int64_t)p.M * p.N > (1LL << 31)) return -1;
   }
-  if (dtype == S4F_F32) {                                  // two tiles a CU, at least eight steps a range
+  if (dtype == S4F_F32) {                                  // two tiles a CU, at least four steps a range
     lay_out(a, BT, BT, BKR, 1, true);
+    const int tiles = a.p[a.count - 1].work_end;
     int steps = 0;
     for (int i = 0; i < a.count; ++i) steps = std::max(steps, a.p[i].steps);
-    const int64_t bytes = lay_out(a, BT, BT, BKR, (int)std::max<int64_t>(1, std::min<int64_t>((512 + a.p[a.count - 1].work_end / 2) / a.p[a.count - 1].work_end, steps / 8)), true);
+    const int64_t bytes = lay_out(a, BT, BT, BKR, std::max(1, std::min(512 / tiles, steps / 4)), true);
     return a.p[a.count - 1].work_end < INT32_MAX ? bytes : -1;
   }
   double best = 0;
@@ -541,7 +531,7 @@ S4F_API int s4f_wgrad_packed(const s4f_wgrad_packed_desc* descs, int count, int 
     return 0;
   }
   const dim3 grid(a.p[count - 1].work_end);
-  hipLaunchKernelGGL(wgrad_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(wgrad_f32_kernel, grid, dim3(256), 0, (hipStream_t)stream, a);
   S4F_LAUNCH_CHECK();
   if (join) {
     hipLaunchKernelGGL(wgrad_join_kernel, dim3((unsigned)std::min<int64_t>((n4 + 255) / 256, 2048)), dim3(256), 0, (hipStream_t)stream, a);
