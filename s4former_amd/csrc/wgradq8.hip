@@ -431,7 +431,7 @@ int64_t lay_out(Args& a, int tm, int tn, int step, int s, bool exact_slabs) {
 int64_t plan(Args& a, int dtype) {
   for (int i = 0; i < a.count; ++i) {
     const Problem& p = a.p[i];
-    if (p.M <= 0 || p.N <= 0 || p.rows <= 0 || p.M % 8 || p.N % ACTQ8_GROUP || p.rows > (1LL << 31) || (int64_t)p.M * p.N > (1LL << 31)) return -1;
+    if (p.M <= 0 || p.N <= 0 || p.rows <= 0 || p.M % 8 || p.N % ACTQ8_GROUP || p.rows >= (1LL << 31) - 128 || (int64_t)p.M * p.N > (1LL << 31)) return -1;
   }
   if (dtype == S4F_F32) {                                  // two tiles a CU, at least four steps a range
     lay_out(a, BT, BT, BKR, 1, true);
@@ -504,10 +504,13 @@ S4F_API int s4f_wgrad_packed(const s4f_wgrad_packed_desc* descs, int count, int 
   for (int i = 0; i < count; ++i) {
     const s4f_wgrad_packed_desc& d = descs[i];
     S4F_CHECK(d.dy && d.codes && d.scales && d.out, "%s: null pointer in problem %d", who, i);
-    S4F_CHECK((uintptr_t)d.dy % 16 == 0 && (uintptr_t)d.codes % 16 == 0 && (uintptr_t)d.out % 16 == 0 && d.lddy >= 0 &&
-                  d.lddy % (dtype == S4F_BF16 ? 8 : 4) == 0 && d.lddy < (1 << 23), "%s: rows of dy, codes and out must start on 16-byte boundaries (problem %d)", who, i);
+    S4F_CHECK((uintptr_t)d.dy % 16 == 0 && (uintptr_t)d.codes % 16 == 0 && (uintptr_t)d.out % 16 == 0 && d.lddy % (dtype == S4F_BF16 ? 8 : 4) == 0,
+              "%s: rows of dy, codes and out must start on 16-byte boundaries (problem %d)", who, i);
     S4F_CHECK(d.M > 0 && d.N > 0 && d.rows > 0 && d.M % 8 == 0 && d.N % ACTQ8_GROUP == 0,
               "%s: M=%d must be a multiple of 8, N=%d of 32, rows=%lld positive", who, d.M, d.N, (long long)d.rows);
+    S4F_CHECK(d.lddy >= d.M, "%s: rows of dy overlap (ld %lld < M %d)", who, (long long)d.lddy, d.M);
+    // (the bf16 kernel addresses 64 rows with 32-bit offsets)
+    S4F_CHECK(d.lddy < (1 << 23) && d.N < (1 << 24) && d.rows < (1LL << 31) - 128, "%s: sizes too large for one launch", who);
     Problem& p = a.p[i];
     p.dy = d.dy; p.lddy = d.lddy; p.codes = d.codes; p.scales = d.scales; p.out = d.out; p.M = d.M; p.N = d.N; p.rows = d.rows;
   }

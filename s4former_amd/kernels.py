@@ -510,6 +510,9 @@ def attention_bwd_fused(qkv, ctx, dctx, lse, delta, dqkv, B, N, H, ws, bias_u=No
 
 # ------------------------------------------------------------------------------------------------ norm + rotation of queries and keys
 # The operators below are also called at sizes where the launch is all there is, so their checks read each attribute of a tensor once.
+_F32T, _I8, _U8 = torch.float32, torch.int8, torch.uint8
+
+
 def _dev(t):
     """the current device's index if t is a device tensor, else an index that no tensor has"""
     return L._cur_device() if t.is_cuda else -2
@@ -559,10 +562,11 @@ def _apart(pa, lda, pb, ldb, rows, row_bytes, es, what):
 
 
 def _launch(name, *args):
-    if L._prof is not None or L._lib is None:
+    lib = L._lib
+    if lib is None or L._prof is not None:
         return call(name, *args)
-    if getattr(L._lib, name)(*args):
-        raise S4FError(f'{name} failed: {L._lib.s4f_last_error().decode(errors="replace")}')
+    if getattr(lib, name)(*args):
+        raise S4FError(f'{name} failed: {lib.s4f_last_error().decode(errors="replace")}')
 
 
 def _stream_of(dev):
@@ -573,9 +577,8 @@ def _gains_tables(rows, gq, gk, cos, sin, dev, what):
     """pointers of the gains and tables (None -> NULL) and the number of positions"""
     if (gq is None) != (gk is None) or (cos is None) != (sin is None):
         raise S4FError(f'{what}: gains (gq, gk) and tables (cos, sin) come in pairs')
-    f32 = torch.float32
     if gq is not None:
-        gq, gk = _vec(gq, f32, 64, dev, what + ' gq'), _vec(gk, f32, 64, dev, what + ' gk')
+        gq, gk = _vec(gq, _F32T, 64, dev, what + ' gq'), _vec(gk, _F32T, 64, dev, what + ' gk')
     elif cos is None:
         raise S4FError(f'{what}: neither a norm (gq, gk) nor a rotation (cos, sin) asked for')
     period = 0
@@ -586,13 +589,13 @@ def _gains_tables(rows, gq, gk, cos, sin, dev, what):
         period = sh[0]
         if period == 0 or rows % period:
             raise S4FError(f'{what}: {period} positions do not divide {rows} rows')
-        cos, sin = _vec(cos, f32, period * 32, dev, what + ' cos'), _vec(sin, f32, period * 32, dev, what + ' sin')
+        cos, sin = _vec(cos, _F32T, period * 32, dev, what + ' cos'), _vec(sin, _F32T, period * 32, dev, what + ' sin')
     return gq, gk, cos, sin, period
 
 
 def _packed_ptrs(packed, rows, C, dev, what):
     codes, scales = packed
-    return _vec(codes, torch.int8, rows * C, dev, what + ' codes'), _vec(scales, torch.uint8, rows * (C // 32), dev, what + ' scales')
+    return _vec(codes, _I8, rows * C, dev, what + ' codes'), _vec(scales, _U8, rows * (C // 32), dev, what + ' scales')
 
 
 def qk_norm_rope_fwd(x, y, Hq, Hk, dtype, gq=None, gk=None, cos=None, sin=None, eps=1e-6, packed=None):
@@ -637,7 +640,7 @@ def qk_norm_rope_bwd(dy, dx, Hq, Hk, dtype, x=None, packed=None, gq=None, gk=Non
     if norm:
         if (x is None) == (packed is None) or dgq is None or dgk is None:
             raise S4FError('qk_norm_rope_bwd: the norm needs x or packed (not both), dgq and dgk')
-        dgqp, dgkp = _vec(dgq, torch.float32, 64, dev, 'qk_norm_rope_bwd dgq'), _vec(dgk, torch.float32, 64, dev, 'qk_norm_rope_bwd dgk')
+        dgqp, dgkp = _vec(dgq, _F32T, 64, dev, 'qk_norm_rope_bwd dgq'), _vec(dgk, _F32T, 64, dev, 'qk_norm_rope_bwd dgk')
         if abs(dgqp - dgkp) < 256:
             raise S4FError('qk_norm_rope_bwd: dgq and dgk overlap')
         if packed is not None:
@@ -668,7 +671,7 @@ def _group_cols(C, what):
 def act_pack(x, codes, scales, dtype):
     """8-bit checkpoint of x [rows, C] (C a multiple of 32; a column slice of a wider buffer qualifies): codes int8 [rows, C], scales uint8
     [rows, C / 32].  |x - restored| <= max |x| / 127.5 over the 32 channels; a group with an infinity or a NaN comes back as NaN."""
-    C, dev = x.shape[-1], _dev(x)
+    C, dev = x.shape[-1] if x.dim() else 0, _dev(x)
     _group_cols(C, 'act_pack')
     xp, ldx, rows = _mat(x, _tdt(dtype), C, dev, 'act_pack x')
     codes, scales = _packed_ptrs((codes, scales), rows, C, dev, 'act_pack')
@@ -678,7 +681,7 @@ def act_pack(x, codes, scales, dtype):
 
 def act_unpack(codes, scales, y, dtype):
     """y [rows, C] = the activation that act_pack put away"""
-    C, dev = y.shape[-1], _dev(y)
+    C, dev = y.shape[-1] if y.dim() else 0, _dev(y)
     _group_cols(C, 'act_unpack')
     yp, ldy, rows = _mat(y, _tdt(dtype), C, dev, 'act_unpack y')
     codes, scales = _packed_ptrs((codes, scales), rows, C, dev, 'act_unpack')
@@ -708,7 +711,7 @@ def wgrad_packed(problems, dtype, ws=None, accumulate=True):
         if ld < M:
             raise S4FError('wgrad_packed dy: the rows overlap')
         cp, sp = _packed_ptrs((codes, scales), rows, N, dev, 'wgrad_packed')
-        op = _vec(out, torch.float32, M * N, dev, 'wgrad_packed out')
+        op = _vec(out, _F32T, M * N, dev, 'wgrad_packed out')
         spans.append((op, op + 4 * M * N))
         if rows:
             descs.append((dyp, ld, cp, sp, op, rows, M, N))

@@ -175,16 +175,26 @@ def layer_backward(sv, prm, g2, B, N, E, H, qk_norm, tabs):
     return g, dx.reshape(B, N, E)
 
 
-@pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
+@pytest.fixture
+def residual(request):
+    from s4former_amd import runtime
+    before = runtime._resid_fp32
+    runtime.set_residual_fp32(request.param == 'fp32')
+    yield request.param
+    runtime.set_residual_fp32(before)
+
+
+@pytest.mark.parametrize('dtype,residual', [('fp32', 'fp32'), ('bf16', 'fp32'), ('bf16', 'bf16')], indirect=['residual'])
 @pytest.mark.parametrize('qk_norm,theta', [(True, 100.0), (False, None), (False, 100.0)])
-def test_backward_from_checkpoints(dtype, qk_norm, theta):
+def test_backward_from_checkpoints(dtype, residual, qk_norm, theta):
     """one layer: its gradients are the formulas' on the activations as the checkpoints restore them"""
     m = make_vit(dtype, layers=1, img=64, qk_norm=qk_norm, rope_theta=theta, act_q8=True)
     x = torch.randn(3, 3, 64, 64, generator=torch.Generator().manual_seed(5)).cuda()
     out = m(x)[0]
     (node,) = saved_layers(out)
     sv = dict(node.sv)
-    assert hasattr(sv['a'], 'codes') and hasattr(sv['x'], 'codes') and (isinstance(sv['pre'], tuple) == qk_norm)
+    assert hasattr(sv['a'], 'codes') and hasattr(sv['x'], 'codes') and sv['x'].dtype == (torch.bfloat16 if residual == 'bf16' else torch.float32)
+    assert isinstance(sv['pre'], tuple) == qk_norm
     B, N, E = 3, 17, 256
     go = torch.randn(out.shape, generator=torch.Generator().manual_seed(8)).to(out.dtype).cuda()
     g2 = torch.zeros(B, N, E, dtype=torch.float64)
