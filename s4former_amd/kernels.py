@@ -605,9 +605,15 @@ def qk_norm_rope_fwd(x, y, Hq, Hk, dtype, gq=None, gk=None, cos=None, sin=None, 
     checkpoint of the pre-norm x that qk_norm_rope_bwd reads."""
     C, T, dev = (Hq + Hk) * 64, _tdt(dtype), _dev(x)
     xp, ldx, rows = _mat(x, T, C, dev, 'qk_norm_rope_fwd x')
-    yp, ldy, yrows = _mat(y, T, C, dev, 'qk_norm_rope_fwd y')
-    if yrows != rows:
-        raise S4FError(f'qk_norm_rope_fwd: x has {rows} rows, y {yrows}')
+    if y is x:
+        yp, ldy = xp, ldx
+    else:
+        yp, ldy, yrows = _mat(y, T, C, dev, 'qk_norm_rope_fwd y')
+        if yrows != rows:
+            raise S4FError(f'qk_norm_rope_fwd: x has {rows} rows, y {yrows}')
+        if xp != yp or ldx != ldy:
+            es = 2 if dtype == BF16 else 4
+            _apart(xp, ldx, yp, ldy, rows, C * es, es, 'qk_norm_rope_fwd: x and y')
     codes = scales = None
     if packed is not None:
         if gq is None:
@@ -616,8 +622,6 @@ def qk_norm_rope_fwd(x, y, Hq, Hk, dtype, gq=None, gk=None, cos=None, sin=None, 
     if rows == 0:
         return
     gq, gk, cos, sin, period = _gains_tables(rows, gq, gk, cos, sin, dev, 'qk_norm_rope_fwd')
-    es = 2 if dtype == BF16 else 4
-    _apart(xp, ldx, yp, ldy, rows, C * es, es, 'qk_norm_rope_fwd: x and y')
     _launch('s4f_qk_norm_rope_fwd', xp, ldx, yp, ldy, gq, gk, cos, sin, period, eps, codes, scales, rows, Hq, Hk, dtype, _stream_of(dev))
 
 
@@ -668,25 +672,37 @@ def _group_cols(C, what):
         raise S4FError(f'{what}: {C} channels are not a positive multiple of 32')
 
 
+def _ckpt(t, codes, scales, dtype, what):
+    """(pointer, row stride, codes, scales, rows, C, device) of an activation and its checkpoint"""
+    sh, dev = t.shape, t.get_device()
+    rows, C = sh if len(sh) == 2 else (0, 0)
+    if (C > 0 and not C & 31 and t.dtype is (torch.bfloat16 if dtype == BF16 else _F32T) and dev >= 0 and dev == L._cur_device() and
+            codes.dtype is _I8 and codes.numel() == rows * C and codes.get_device() == dev and codes.is_contiguous() and
+            scales.dtype is _U8 and scales.numel() == rows * (C >> 5) and scales.get_device() == dev and scales.is_contiguous()):
+        ld, one = t.stride()
+        if one == 1:
+            return t.data_ptr(), ld if rows > 1 else C, codes.data_ptr(), scales.data_ptr(), rows, C, dev
+    # something is wrong: say what
+    _group_cols(C, what)
+    dev = _dev(t)
+    _mat(t, _tdt(dtype), C, dev, what)
+    _packed_ptrs((codes, scales), rows, C, dev, what)
+    raise S4FError(f'{what}: unsupported arguments')
+
+
 def act_pack(x, codes, scales, dtype):
     """8-bit checkpoint of x [rows, C] (C a multiple of 32; a column slice of a wider buffer qualifies): codes int8 [rows, C], scales uint8
     [rows, C / 32].  |x - restored| <= max |x| / 127.5 over the 32 channels; a group with an infinity or a NaN comes back as NaN."""
-    C, dev = x.shape[-1] if x.dim() else 0, _dev(x)
-    _group_cols(C, 'act_pack')
-    xp, ldx, rows = _mat(x, _tdt(dtype), C, dev, 'act_pack x')
-    codes, scales = _packed_ptrs((codes, scales), rows, C, dev, 'act_pack')
+    xp, ldx, cp, sp, rows, C, dev = _ckpt(x, codes, scales, dtype, 'act_pack')
     if rows:
-        _launch('s4f_act_pack', xp, ldx, codes, scales, rows, C, dtype, _stream_of(dev))
+        _launch('s4f_act_pack', xp, ldx, cp, sp, rows, C, dtype, _stream_of(dev))
 
 
 def act_unpack(codes, scales, y, dtype):
     """y [rows, C] = the activation that act_pack put away"""
-    C, dev = y.shape[-1] if y.dim() else 0, _dev(y)
-    _group_cols(C, 'act_unpack')
-    yp, ldy, rows = _mat(y, _tdt(dtype), C, dev, 'act_unpack y')
-    codes, scales = _packed_ptrs((codes, scales), rows, C, dev, 'act_unpack')
+    yp, ldy, cp, sp, rows, C, dev = _ckpt(y, codes, scales, dtype, 'act_unpack')
     if rows:
-        _launch('s4f_act_unpack', codes, scales, yp, ldy, rows, C, dtype, _stream_of(dev))
+        _launch('s4f_act_unpack', cp, sp, yp, ldy, rows, C, dtype, _stream_of(dev))
 
 
 def wgrad_packed_ws_bytes(problems, dtype):
