@@ -27,12 +27,12 @@ struct Problem {
 struct Args { Problem p[MAXP]; int count, accumulate, variant; };
 
 // ------------------------------------------------------------------------------------------------- fp32
-// 64 x 64 tile, four waves of 32 x 32, 32 rows a step, two buffers; several tiles a CU hide the latency of loads and reads.  The fp32
-// matrix rate (256 operations a clock and CU) bounds large problems; the small tile keeps ragged sizes from wasting it.
-constexpr int BT = 64, BKR = 32, LDF = BT * 4 + 16;      // bytes of a row in LDS: rows 4 apart lie 16 banks apart
+// 64 x 64 tile, four waves of 32 x 32, 64 rows a step, two buffers, two tiles a CU.  The fp32 matrix rate (256 operations a clock and CU)
+// bounds large problems; the small tile keeps ragged sizes from wasting it, the long step covers the latency of the next one's loads.
+constexpr int BT = 64, BKR = 64, LDF = BT * 4 + 16;      // bytes of a row in LDS: rows 4 apart lie 16 banks apart
 
 __global__ __launch_bounds__(256) void wgrad_f32_kernel(const Args args) {
-  __shared__ __attribute__((aligned(16))) char la[2][BKR * LDF], lb[2][BKR * LDF];
+  __shared__ __attribute__((aligned(16))) char la[2][BKR * LDF], lb[2][BKR * LDF];      // 68 KiB
   int which = 0;
   for (int i = 0; i < MAXP - 1; ++i) which += i < args.count - 1 && (int)blockIdx.x >= args.p[i].work_end ? 1 : 0;
   const Problem& P = args.p[which];
@@ -44,8 +44,8 @@ __global__ __launch_bounds__(256) void wgrad_f32_kernel(const Args args) {
 
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, g = l >> 4, li = l & 15;
   const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-  // a thread's chunks: rows tid / 16 and + 16 of dY, four values; row tid / 8 of the codes, eight values (M is a multiple of 8 and N of
-  // 32: a chunk is inside or outside)
+  // a thread's chunks: rows tid / 16 (+ 16 ..) of dY, four values; rows tid / 8 and + 32 of the codes, eight values (M is a multiple of 8
+  // and N of 32: a chunk is inside or outside)
   const int ra = tid >> 4, ca = (tid & 15) * 4, rb = tid >> 3, cb = (tid & 7) * 8;
   const bool aok = m0 + ca < M, bok = n0 + cb < N;
   const float* pa = reinterpret_cast<const float*>(P.dy) + ((int64_t)k_beg * BKR + ra) * P.lddy + m0 + ca;
@@ -53,26 +53,33 @@ __global__ __launch_bounds__(256) void wgrad_f32_kernel(const Args args) {
   const uint8_t* ps = P.scales + ((int64_t)k_beg * BKR + rb) * (N / ACTQ8_GROUP) + (n0 + cb) / ACTQ8_GROUP;
   int64_t left = P.rows - (int64_t)k_beg * BKR;            // rows from the step on
 
-  chunk16 xa[2];
-  uint2 xb;
-  uint32_t xs;
+  constexpr int NA = BKR / 16, NB = BKR / 32;
+  chunk16 xa[NA];
+  uint2 xb[NB];
+  uint32_t xs[NB];
   auto load = [&]() {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) xa[i] = aok && ra + 16 * i < left ? ld_global16(pa + (int64_t)(16 * i) * P.lddy) : zero16();
-    const bool ok = bok && rb < left;
-    xb = ok ? *reinterpret_cast<const uint2*>(pb) : make_uint2(0, 0);
-    xs = ok ? *ps : 0u;
+    for (int i = 0; i < NA; ++i) xa[i] = aok && ra + 16 * i < left ? ld_global16(pa + (int64_t)(16 * i) * P.lddy) : zero16();
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const bool ok = bok && rb + 32 * i < left;
+      xb[i] = ok ? *reinterpret_cast<const uint2*>(pb + (int64_t)(32 * i) * N) : make_uint2(0, 0);
+      xs[i] = ok ? ps[(int64_t)(32 * i) * (N / ACTQ8_GROUP)] : 0u;
+    }
     pa += (int64_t)BKR * P.lddy; pb += (int64_t)BKR * N; ps += (int64_t)BKR * (N / ACTQ8_GROUP); left -= BKR;
   };
   auto store = [&](int buf) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) *reinterpret_cast<chunk16*>(la[buf] + (ra + 16 * i) * LDF + ca * 4) = xa[i];
-    const float s = q8_scale(xs);
-    f32x4 v0, v1;
+    for (int i = 0; i < NA; ++i) *reinterpret_cast<chunk16*>(la[buf] + (ra + 16 * i) * LDF + ca * 4) = xa[i];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { v0[e] = q8_code(xb.x, e) * s; v1[e] = q8_code(xb.y, e) * s; }
-    *reinterpret_cast<f32x4*>(lb[buf] + rb * LDF + cb * 4) = v0;
-    *reinterpret_cast<f32x4*>(lb[buf] + rb * LDF + cb * 4 + 16) = v1;
+    for (int i = 0; i < NB; ++i) {
+      const float s = q8_scale(xs[i]);
+      f32x4 v0, v1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { v0[e] = q8_code(xb[i].x, e) * s; v1[e] = q8_code(xb[i].y, e) * s; }
+      *reinterpret_cast<f32x4*>(lb[buf] + (rb + 32 * i) * LDF + cb * 4) = v0;
+      *reinterpret_cast<f32x4*>(lb[buf] + (rb + 32 * i) * LDF + cb * 4 + 16) = v1;
+    }
   };
 
   f32x4 acc[2][2];
@@ -85,16 +92,19 @@ __global__ __launch_bounds__(256) void wgrad_f32_kernel(const Args args) {
     const int buf = (k - k_beg) & 1;
     if (k + 1 < k_end) load();
     __syncthreads();
-    Frag<float> a[2], b[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      lds_read_tr(a[i], la[buf], LDF, 0, wm + i * 16);
-      lds_read_tr(b[i], lb[buf], LDF, 0, wn + i * 16);
+    for (int h = 0; h < BKR; h += 32) {
+      Frag<float> a[2], b[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        lds_read_tr(a[i], la[buf], LDF, h, wm + i * 16);
+        lds_read_tr(b[i], lb[buf], LDF, h, wn + i * 16);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mma16(a[i], b[j], acc[i][j]);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mma16(a[i], b[j], acc[i][j]);
     if (k + 1 < k_end) store(buf ^ 1);                     // (last read in the step before: everyone has passed the barrier since)
   }
 
@@ -433,12 +443,14 @@ int64_t plan(Args& a, int dtype) {
     const Problem& p = a.p[i];
     if (p.M <= 0 || p.N <= 0 || p.rows <= 0 || p.M % 8 || p.N % ACTQ8_GROUP || p.rows >= (1LL << 31) - 128 || (int64_t)p.M * p.N > (1LL << 31)) return -1;
   }
-  if (dtype == S4F_F32) {                                  // two tiles a CU, at least four steps a range
+  if (dtype == S4F_F32) {
+    // two tiles a CU, four where a range keeps sixteen steps (520 x 416 over 2,307 rows: 24 us with 8 ranges of 5 steps, 28 with 13 of 3;
+    // 768 x 768 over 16,400: 238 us with 3 of 86, 209 with 7 of 37)
     lay_out(a, BT, BT, BKR, 1, true);
     const int tiles = a.p[a.count - 1].work_end;
     int steps = 0;
     for (int i = 0; i < a.count; ++i) steps = std::max(steps, a.p[i].steps);
-    const int64_t bytes = lay_out(a, BT, BT, BKR, std::max(1, std::min(512 / tiles, steps / 4)), true);
+    const int64_t bytes = lay_out(a, BT, BT, BKR, std::max(1, std::min(1024 / tiles, std::max(512 / tiles, steps / 16))), true);
     return a.p[a.count - 1].work_end < INT32_MAX ? bytes : -1;
   }
   double best = 0;
