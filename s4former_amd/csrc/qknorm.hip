@@ -11,6 +11,10 @@
 // a rotation's pair stays in the lane, the mean takes two or three lane exchanges, and one 8-bit group (32 channels: a half) is
 // spread over the same lanes.  Both passes are bound by HBM; the tables (256 bytes a row) are read per head but come from cache,
 // the heads of a row being neighbours in the grid.
+//
+// Measured, bf16, 16,400 rows x 24 heads: forward 17.4 us with the tensors in the last-level cache (6.0 TB/s) and 23.3 us on fresh ones
+// (4.5 TB/s; a large copy reaches 4.8 - 5.0), with the checkpoint 21.9 us; backward 25.7 us from the checkpoint and 27.7 us from x,
+// 4 us of them the join of the gains.  A call on few rows takes 2.5 - 3.5 us on the GPU, less than its launch costs the host.
 #include "actq8.h"
 #include "../../include/s4f.h"
 #include <algorithm>

@@ -4,7 +4,7 @@
 // units.  Up to four problems (the layers of one encoder block) share a grid.
 //
 // The rows are cut into ranges so that the grid fills the chip; a range's sums go to a slab of the workspace with plain stores and
-// wgrad_join_kernel adds the slabs in the order of the ranges: the result does not depend on timing.
+// a second kernel adds the slabs in the order of the ranges: the result does not depend on timing.
 #include "actq8.h"
 #include "../../include/s4f.h"
 #include <algorithm>
@@ -19,12 +19,19 @@ struct Problem {
   const void* dy; int64_t lddy;
   const int8_t* codes; const uint8_t* scales;
   float* out;                            // [M][N]
-  float* slab;                           // [splits][M][N], splits > 1
+  float* slab;                           // splits > 1: partial sums, [splits][M][N] (fp32) or [splits][tiles] in register order (bf16)
   int64_t rows;
   int M, N, tiles_n, tiles, splits, steps, steps_per_split;
   int work_end;                          // running sum of tiles x splits
 };
 struct Args { Problem p[MAXP]; int count, accumulate, variant; };
+
+// Work is numbered (problem, row range, tile).  Consecutive blocks go to the eight XCDs in turn; a contiguous eighth of the numbers a
+// XCD lets the tiles of a row range, which read the same rows of dY and X, meet in one L2.
+__device__ __forceinline__ int work_of_block(int total) {
+  const int xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
+  return min(xcd, r8) * (q8 + 1) + max(xcd - r8, 0) * q8 + ((int)blockIdx.x >> 3);
+}
 
 // ------------------------------------------------------------------------------------------------- fp32
 // 64 x 64 tile, four waves of 32 x 32, 64 rows a step, two buffers, two tiles a CU.  The fp32 matrix rate (256 operations a clock and CU)
@@ -33,10 +40,11 @@ constexpr int BT = 64, BKR = 64, LDF = BT * 4 + 16;      // bytes of a row in LD
 
 __global__ __launch_bounds__(256) void wgrad_f32_kernel(const Args args) {
   __shared__ __attribute__((aligned(16))) char la[2][BKR * LDF], lb[2][BKR * LDF];      // 68 KiB
+  const int w = work_of_block(args.p[args.count - 1].work_end);
   int which = 0;
-  for (int i = 0; i < MAXP - 1; ++i) which += i < args.count - 1 && (int)blockIdx.x >= args.p[i].work_end ? 1 : 0;
+  for (int i = 0; i < MAXP - 1; ++i) which += i < args.count - 1 && w >= args.p[i].work_end ? 1 : 0;
   const Problem& P = args.p[which];
-  const int local = (int)blockIdx.x - (which ? args.p[which - 1].work_end : 0);
+  const int local = w - (which ? args.p[which - 1].work_end : 0);
   const int z = local / P.tiles, tile = local - z * P.tiles;
   const int m0 = tile / P.tiles_n * BT, n0 = tile % P.tiles_n * BT;
   const int k_beg = z * P.steps_per_split, k_end = min(k_beg + P.steps_per_split, P.steps);
@@ -127,19 +135,23 @@ __global__ __launch_bounds__(256) void wgrad_f32_kernel(const Args args) {
 }
 
 // ------------------------------------------------------------------------------------------------- bf16
-// Tile (64 MI) x (64 NI), four waves in 2 x 2, each MI x NI products of 32 x 32 x 16; 64 rows of dY and X a step, two buffers in LDS.
-// One wave per SIMD holds the sums of a quarter of the tile, so that a fragment read feeds four products (at 256 x 256): with eight
-// waves LDS would bound the loop.  A wave alone on its SIMD has to keep the matrix unit busy by itself, so every read, store and
-// conversion stands between products:
+// Tile (32 MI WM) x (32 NI WN), WM x WN waves with MI x NI products of 32 x 32 x 16 each; 64 rows of dY and X a step, two buffers in LDS.
+// dY goes to LDS without a stop in registers; codes wait about two steps in registers and become bf16 on their way to LDS.
 //   barrier (step k's buffer is complete, the other one free)
-//   part 0: products of step k - 1's last 16 rows, reads of the fragments of step k's rows 0 .. 15
+//   part 0: products of step k - 1's last 16 rows, reads of the fragments of step k's rows 0 .. 15, loads of the dY of step k + 1
 //   parts 1 - 3: products of 16 rows of step k, reads of the next 16
-// Parts 0 - 2 also store a third each of step k + 1 (in registers since about two steps; codes become bf16 on the way) into the other
-// buffer and load what takes its registers' place; part 3 reads early and stores nothing, so that nothing is left to wait for at
-// the barrier, and the products behind the barrier have their fragments in registers.
+// Parts 0 - 2 also store a third each of step k + 1's X into the other buffer and load what takes its registers' place; part 3 reads
+// early and stores nothing, so that nothing is left to wait for at the barrier, and the products behind the barrier have their
+// fragments in registers.  Reads, conversions and loads stand between the products in the order written.
+//
+// Measured at 256 x 256: 1.21 us a step on part of the chip (70 % of the matrix rate at 2.4 GHz), 1.65 us with every CU at work, where
+// the power of the matrix units lowers the clock to about 1.8 GHz: 4096 x 4096 over 16,384 rows take 421 us, 1,305 TFLOP/s; a large
+// library product of bf16 matrices reaches 1,600 on this card, this kernel without its conversions and loads about 1,550.  No bank
+// conflicts are counted.  Not faster: four waves with 128 x 128 each (1.38 us a step: a store blocks the wave that also has to feed the
+// matrix unit), a third buffer of dY, the conversions spread over all four parts; touching dY's lines a step ahead costs 15 %.
 //
 // LDS image: [64 rows][columns] bf16, the 64-byte unit u of row r at u ^ (r & 3): the four rows x 64 bytes that half a wave reads in
-// one transposing read lie in different banks, and so do the stores.
+// one transposing read lie in different banks, and so do the stores (served eight lanes at a time).
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
@@ -166,10 +178,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args 
   // one object a buffer: the compiler then sees that a read of one does not wait for what arrives in another
   __shared__ __attribute__((aligned(1024))) char A0[STEP * RA], A1[STEP * RA], B0[STEP * RB], B1[STEP * RB];
 
-  // block -> (problem, row range, tile), consecutive ones on one XCD: the tiles of a row range read the same rows of dY and X
-  const int total = args.p[args.count - 1].work_end;
-  const int xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
-  const int w = min(xcd, r8) * (q8 + 1) + max(xcd - r8, 0) * q8 + (blockIdx.x >> 3);
+  const int w = work_of_block(args.p[args.count - 1].work_end);
   int which = 0;
   for (int i = 0; i < MAXP - 1; ++i) which += i < args.count - 1 && w >= args.p[i].work_end ? 1 : 0;
   const Problem& P = args.p[which];
@@ -183,9 +192,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args 
   const int wm = wave / WN, wn = wave % WN;
 
   // ---- global side: chunk i of a thread is DA (DB) rows below chunk i - 1.  The resources cover the rows of the step, so rows behind
-  // the range read as zero; columns outside are given an offset beyond every resource.  16 codes come as two loads of 8: the lanes
-  // whose chunk lies in the upper 256 bytes of a 512-byte span of LDS take (and store) the upper half first, so that the 16 lanes of
-  // one 16-byte store touch every bank once
+  // the range read as zero; columns outside are given an offset beyond every resource.  16 codes come as two loads of 8: four of each
+  // eight lanes take (and store) the upper half first, so that the eight 16-byte stores served at once touch different banks
   const int ra = tid / CA, ua = (tid % CA >> 2) ^ (ra & 3), ca = 4 * ua + (tid & 3), rb = tid / CB, cb = tid % CB, hb = (tid >> 2) & 1;
   const int OUT = (int)0x80000000;
   const int ld2 = (int)(P.lddy * 2), ns = N / ACTQ8_GROUP;
