@@ -733,13 +733,15 @@ def wgrad_packed(problems, dtype, ws=None, accumulate=True):
             descs.append((dyp, ld, cp, sp, op, rows, M, N))
         elif not accumulate:
             out.zero_()
+    wsp, wsb = _buf(ws, dev, 'wgrad_packed ws')
+    if wsb:
+        spans.append((wsp, wsp + wsb))
     if len(spans) > 1:
         spans.sort()
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise S4FError('wgrad_packed: the outputs overlap')
+            raise S4FError('wgrad_packed: outputs (or an output and the workspace) overlap')
     if not descs:
         return
-    wsp, wsb = _buf(ws, dev, 'wgrad_packed ws')
     arr = (L.WgradPackedDesc * len(descs))(*descs)
     _launch('s4f_wgrad_packed', arr, len(descs), dtype, 1 if accumulate else 0, wsp, wsb, _stream_of(dev))
 

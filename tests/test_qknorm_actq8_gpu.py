@@ -468,3 +468,177 @@ def test_chain_in_a_graph(K, code):
         torch.cuda.synchronize()
         for k in OUTS:
             assert torch.equal(new[k], st[k]), (i, k)
+
+
+# ------------------------------------------------------------------------------------------------------------- far ends of the calls
+@pytest.mark.parametrize('code', DTYPES)
+def test_offsets_beyond_32_bits(K, code):
+    """slices of a buffer whose last rows lie more than 2^32 elements behind the first"""
+    rows, ld, t = 70001, 65536, tdt(code)
+    buf = torch.empty(rows, ld, device='cuda', dtype=t)
+    pick = torch.tensor([0, 1, 32767, 32768, 65535, 65536, rows - 2, rows - 1], device='cuda')
+    x, y = buf[:, 64:64 + 256], buf[:, 1024:1024 + 256]
+    x.copy_(torch.randn(rows, 256, device='cuda', generator=torch.Generator(device='cuda').manual_seed(1)).to(t))
+    g = [torch.rand(64, device='cuda') + 0.5 for _ in range(2)]
+    codes, scales = torch.empty(rows, 256, device='cuda', dtype=torch.int8), torch.empty(rows, 8, device='cuda', dtype=torch.uint8)
+    K.qk_norm_rope_fwd(x, y, 2, 2, code, gq=g[0], gk=g[1], packed=(codes, scales))
+    few = x[pick].contiguous()
+    ref = torch.empty_like(few)
+    c2, s2 = torch.empty(len(pick), 256, device='cuda', dtype=torch.int8), torch.empty(len(pick), 8, device='cuda', dtype=torch.uint8)
+    K.qk_norm_rope_fwd(few, ref, 2, 2, code, gq=g[0], gk=g[1], packed=(c2, s2))
+    assert torch.equal(y[pick], ref) and torch.equal(codes[pick], c2) and torch.equal(scales[pick], s2)
+    K.act_pack(x, codes, scales, code)
+    assert torch.equal(codes[pick], c2) and torch.equal(scales[pick], s2)
+    K.act_unpack(codes, scales, y, code)
+    r2 = torch.empty_like(few)
+    K.act_unpack(c2, s2, r2, code)
+    assert torch.equal(y[pick], r2)
+    dx = torch.empty(rows, 256, device='cuda', dtype=t)
+    dg = [torch.empty(64, device='cuda') for _ in range(4)]
+    ws = torch.empty(K.qk_norm_rope_ws_bytes(rows, 2, 2), device='cuda', dtype=torch.uint8)
+    kw = dict(gq=g[0], gk=g[1], accumulate=False, ws=ws)
+    K.qk_norm_rope_bwd(x, dx, 2, 2, code, x=x, dgq=dg[0], dgk=dg[1], **kw)
+    d2 = torch.empty_like(few)
+    K.qk_norm_rope_bwd(few, d2, 2, 2, code, x=few, dgq=dg[2], dgk=dg[3], **kw)
+    assert torch.equal(dx[pick], d2)
+    # weight gradients: everything but the picked rows is zero, so the sums are those of the picked rows
+    dy = buf[:, 2048:2048 + 64]
+    dy.zero_()
+    some = torch.randn(len(pick), 64, device='cuda', generator=torch.Generator(device='cuda').manual_seed(2)).to(t)
+    dy[pick] = some
+    outs = [torch.empty(64, 256, device='cuda') for _ in range(2)]
+    wsw = torch.empty(max(16, K.wgrad_packed_ws_bytes([(64, 256, rows)], code)), device='cuda', dtype=torch.uint8)
+    K.wgrad_packed([(dy, codes, scales, outs[0])], code, wsw, accumulate=False)
+    x64 = r2.cpu().double()
+    want, mag = some.cpu().double().t() @ x64, some.cpu().double().abs().t() @ x64.abs()
+    within(outs[0], want, 2 * (len(pick) + 80) * U * mag, 'dW')
+
+
+@pytest.mark.parametrize('code', DTYPES)
+def test_one_long_row_set_of_codes(K, code):
+    """more than 2^31 values in one contiguous tensor"""
+    rows, C, t = 66000, 32768 + 32, tdt(code)
+    assert rows * C > 2 ** 31
+    x = torch.zeros(rows, C, device='cuda', dtype=t)
+    pick = torch.tensor([0, 1, 32000, 65000, rows - 1], device='cuda')
+    few = torch.randn(len(pick), C, device='cuda', generator=torch.Generator(device='cuda').manual_seed(3)).to(t)
+    x[pick] = few
+    codes, scales = torch.empty(rows, C, device='cuda', dtype=torch.int8), torch.empty(rows, C // 32, device='cuda', dtype=torch.uint8)
+    K.act_pack(x, codes, scales, code)
+    c2, s2 = torch.empty(len(pick), C, device='cuda', dtype=torch.int8), torch.empty(len(pick), C // 32, device='cuda', dtype=torch.uint8)
+    K.act_pack(few, c2, s2, code)
+    assert torch.equal(codes[pick], c2) and torch.equal(scales[pick], s2)
+    K.act_unpack(codes, scales, x, code)
+    r2 = torch.empty_like(few)
+    K.act_unpack(c2, s2, r2, code)
+    assert torch.equal(x[pick], r2)
+
+
+@pytest.mark.parametrize('code', DTYPES)
+def test_nan_and_infinity_stay_in_their_head(K, code):
+    case = (1, 6, 3, 2, True, True, False, 0)
+    x, dy, gq, gk, cos, sin = qk_inputs(case, code, seed=70)
+    bad = x.clone()
+    bad[2, 64 + 5] = float('nan')
+    bad[4, 3 * 64 + 40] = float('inf')
+    hit = torch.zeros(6, 5, dtype=torch.bool)
+    hit[2, 1] = hit[4, 3] = True
+    par = dict(gq=cu(gq), gk=cu(gk), cos=cu(cos), sin=cu(sin), eps=1e-6)
+    ys, dxs = [], []
+    ws = torch.empty(K.qk_norm_rope_ws_bytes(6, 3, 2), device='cuda', dtype=torch.uint8)
+    for v in (x, bad):
+        v = v.to(tdt(code)).cuda()
+        y, dx = torch.empty_like(v), torch.empty_like(v)
+        pk = (torch.empty(6, 320, device='cuda', dtype=torch.int8), torch.empty(6, 10, device='cuda', dtype=torch.uint8))
+        K.qk_norm_rope_fwd(v, y, 3, 2, code, packed=pk, **par)
+        dg = [torch.zeros(64, device='cuda') for _ in range(2)]
+        K.qk_norm_rope_bwd(dy.to(tdt(code)).cuda(), dx, 3, 2, code, packed=pk, dgq=dg[0], dgk=dg[1], ws=ws, **par)
+        ys.append(y.cpu().reshape(6, 5, 64)); dxs.append(dx.cpu().reshape(6, 5, 64))
+    for a, b in (ys, dxs):
+        assert torch.equal(a[~hit], b[~hit])
+        assert bool(b[hit].isnan().any(-1).all())
+
+
+@pytest.mark.parametrize('code', DTYPES)
+def test_rows_behind_the_last_stay(K, code):
+    t = tdt(code)
+    big = torch.full((9, 256), 3.0, device='cuda', dtype=t)
+    x = rnd(5, 256, seed=1).to(t).cuda()
+    g = torch.ones(64, device='cuda')
+    K.qk_norm_rope_fwd(x, big[:5], 2, 2, code, gq=g, gk=g)
+    assert bool((big[5:] == 3).all()) and not bool((big[:5] == 3).any())
+    dg = [torch.zeros(64, device='cuda') for _ in range(2)]
+    big.fill_(3.0)
+    K.qk_norm_rope_bwd(x, big[:5], 2, 2, code, x=x, gq=g, gk=g, dgq=dg[0], dgk=dg[1],
+                       ws=torch.empty(K.qk_norm_rope_ws_bytes(5, 2, 2), device='cuda', dtype=torch.uint8))
+    assert bool((big[5:] == 3).all())
+
+
+@pytest.mark.parametrize('code', DTYPES)
+def test_two_graphs_share_their_workspaces(K, code):
+    a, b = _chain_state(K, code, 11), _chain_state(K, code, 12)
+    b['ws'], b['wsw'] = a['ws'], a['wsw']
+    graphs = []
+    for st in (a, b):
+        _chain(K, st, code)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            _chain(K, st, code)
+        graphs.append(g)
+    want = []
+    for st in (a, b):
+        _chain(K, st, code)
+        torch.cuda.synchronize()
+        want.append({k: st[k].clone() for k in OUTS})
+    for _ in range(3):
+        for st in (a, b):
+            for k in OUTS:
+                st[k].zero_()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for w, st in zip(want, (a, b)):
+            for k in OUTS:
+                assert torch.equal(w[k], st[k]), k
+
+
+def test_refusals_on_the_device(K):
+    """what only device tensors reach: overlapping arguments, strides and alignments the kernels do not take, short workspaces"""
+    from s4former_amd._lib import S4FError
+    z = lambda *s, dtype=torch.float32: torch.zeros(*s, device='cuda', dtype=dtype)                      # noqa: E731
+    g, buf = z(64), z(9, 400)
+    i8, u8 = lambda *s: z(*s, dtype=torch.int8), lambda *s: z(*s, dtype=torch.uint8)                     # noqa: E731
+    flat = z(4096)
+    out = z(16, 64)
+    ok = (z(200, 8), i8(200, 64), u8(200, 2))
+    for what, call in {
+        'partly overlapping x and y': lambda: K.qk_norm_rope_fwd(buf[:4, :128], buf[:4, 64:192], 1, 1, 0, gq=g, gk=g),
+        'shifted rows': lambda: K.qk_norm_rope_fwd(buf[:4, :128], buf[1:5, :128], 1, 1, 0, gq=g, gk=g),
+        'misaligned columns': lambda: K.qk_norm_rope_fwd(buf[:4, 1:129], z(4, 128), 1, 1, 0, gq=g, gk=g),
+        'misaligned row stride': lambda: K.act_pack(z(4, 66)[:, :64], i8(4, 64), u8(4, 2), 0),
+        'elements of a row apart': lambda: K.act_pack(z(4, 128)[:, ::2], i8(4, 64), u8(4, 2), 0),
+        'transposed': lambda: K.act_pack(z(64, 64).t(), i8(64, 64), u8(64, 2), 0),
+        'rows of y overlap': lambda: K.act_unpack(i8(4, 64), u8(4, 2), flat.as_strided((4, 64), (16, 1)), 0),
+        'codes of another size': lambda: K.act_pack(z(4, 64), i8(5, 64), u8(4, 2), 0),
+        'codes of another type': lambda: K.act_pack(z(4, 64), u8(4, 64), u8(4, 2), 0),
+        'codes with gaps': lambda: K.act_pack(z(4, 64), i8(4, 128)[:, :64], u8(4, 2), 0),
+        'tables that do not divide the rows': lambda: K.qk_norm_rope_fwd(z(4, 128), z(4, 128), 1, 1, 0, cos=z(3, 32), sin=z(3, 32)),
+        'tables of another width': lambda: K.qk_norm_rope_fwd(z(4, 128), z(4, 128), 1, 1, 0, cos=z(4, 64), sin=z(4, 64)),
+        'tables of different lengths': lambda: K.qk_norm_rope_fwd(z(4, 128), z(4, 128), 1, 1, 0, cos=z(4, 32), sin=z(2, 32)),
+        'half a norm': lambda: K.qk_norm_rope_fwd(z(4, 128), z(4, 128), 1, 1, 0, gq=g),
+        'gains in another type': lambda: K.qk_norm_rope_fwd(z(4, 128), z(4, 128), 1, 1, 0, gq=g.bfloat16(), gk=g.bfloat16()),
+        'checkpoint without the norm': lambda: K.qk_norm_rope_fwd(z(4, 128), z(4, 128), 1, 1, 0, cos=z(4, 32), sin=z(4, 32), packed=(i8(4, 128), u8(4, 4))),
+        'no workspace': lambda: K.qk_norm_rope_bwd(z(4, 128), z(4, 128), 1, 1, 0, x=z(4, 128), gq=g, gk=g, dgq=z(64), dgk=z(64)),
+        'one gain gradient for both': lambda: K.qk_norm_rope_bwd(z(4, 128), z(4, 128), 1, 1, 0, x=z(4, 128), gq=g, gk=g, dgq=g, dgk=g, ws=z(4096)),
+        'x and its checkpoint': lambda: K.qk_norm_rope_bwd(z(4, 128), z(4, 128), 1, 1, 0, x=z(4, 128), packed=(i8(4, 128), u8(4, 4)), gq=g, gk=g, dgq=z(64),
+                                                           dgk=z(64), ws=z(4096)),
+        'one output twice': lambda: K.wgrad_packed([(z(200, 16), *ok[1:], out), (z(200, 16), *ok[1:], out)], 0, z(1 << 16)),
+        'outputs that overlap': lambda: K.wgrad_packed([(z(200, 8), *ok[1:], out[:8]), (z(200, 16), *ok[1:], out)], 0, z(1 << 16)),
+        'output in the workspace': lambda: K.wgrad_packed([(*ok, flat[:512].view(8, 64))], 0, flat),
+        'broadcast rows of dy': lambda: K.wgrad_packed([(z(1, 8).expand(200, 8), *ok[1:], z(8, 64))], 0, z(1 << 16)),
+        'short workspace': lambda: K.wgrad_packed([(z(4000, 64), i8(4000, 64), u8(4000, 2), z(64, 64))], 0, z(4)),
+    }.items():
+        with pytest.raises(S4FError):
+            call()
+            pytest.fail(f'not refused: {what}')
