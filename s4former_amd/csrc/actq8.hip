@@ -108,7 +108,7 @@ int check_extent(const char* who, const void* t, int64_t ld, const void* codes, 
   const int ts = dtype == S4F_BF16 ? 2 : 4;
   S4F_CHECK(ld >= 0 && (ld * ts) % 16 == 0 && (uintptr_t)t % 16 == 0 && (uintptr_t)codes % 16 == 0, "%s: rows and codes must start on 16-byte boundaries", who);
   const int64_t cpr = C / (16 / ts);
-  S4F_CHECK(rows <= (int64_t)0x7fffffff * 1024 / cpr, "%s: rows=%lld too large for one launch", who, (long long)rows);
+  S4F_CHECK(rows <= (int64_t)0xffffff * 256 * UNR / cpr, "%s: rows=%lld too large for one launch", who, (long long)rows);
   S4F_CHECK(ld == C || rows <= (int64_t)0xffffffffu / cpr, "%s: rows=%lld too large for a strided view", who, (long long)rows);
   return 0;
 }

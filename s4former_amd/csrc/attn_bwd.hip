@@ -820,7 +820,7 @@ S4F_API int64_t s4f_workspace_bytes(int op, const int64_t* dims, int ndims) {
     case S4F_WS_ATTENTION_BWD: return ndims == 3 ? s4f_attention_bwd_ws_bytes((int)dims[0], (int)dims[1], (int)dims[2]) : -1;
     case S4F_WS_BN_SUMS: return ndims == 1 && dims[0] > 0 ? 2 * dims[0] * 4 : -1;
     case S4F_WS_GEMM_SPLITK: return ndims == 2 && dims[0] > 0 && dims[1] > 0 ? dims[0] * dims[1] * 4 : -1;
-    case S4F_WS_QK_NORM: return ndims == 3 && dims[1] <= INT32_MAX && dims[2] <= INT32_MAX ? s4f_qk_ws_bytes(dims[0], (int)dims[1], (int)dims[2]) : -1;
+    case S4F_WS_QK_NORM: return ndims == 3 && dims[1] > 0 && dims[1] <= INT32_MAX && dims[2] > 0 && dims[2] <= INT32_MAX ? s4f_qk_ws_bytes(dims[0], (int)dims[1], (int)dims[2]) : -1;
     case S4F_WS_WGRAD_PACKED: return s4f_wgrad_packed_ws(dims, ndims);
     default: return -1;
   }

@@ -18,6 +18,7 @@
 #include "actq8.h"
 #include "../../include/s4f.h"
 #include <algorithm>
+#include <cfloat>
 
 namespace {
 
@@ -246,8 +247,8 @@ __global__ __launch_bounds__(256) void qk_gain_kernel(const float* __restrict__ 
 // blocks of the backward for the heads of one kind: 1,024 in all at most, in proportion, each with at least one full turn of its lanes.
 // (Measured at 16,400 rows x 24 heads, bf16: 512 a kind 25.8 us, 384 26.3, 1,024 26.8, 2,048 30.2: the blocks end with a reduction and
 // leave 256 bytes each to be joined.)
-int bwd_blocks(int64_t rows, int heads, int all, int per) {
-  const int64_t b = (rows * heads + per - 1) / per, cap = std::max(1, 1024 * heads / all);
+int bwd_blocks(int64_t rows, int64_t heads, int64_t all, int per) {
+  const int64_t b = (rows * heads + per - 1) / per, cap = std::max<int64_t>(1, (int64_t)1024 * heads / all);
   return (int)std::min(b, cap);
 }
 
@@ -255,10 +256,11 @@ int check_qk(const char* who, int64_t rows, int Hq, int Hk, int dtype, const flo
              const float* sin, int64_t period, float eps) {
   S4F_CHECK(dtype == S4F_F32 || dtype == S4F_BF16, "%s: bad dtype %d", who, dtype);
   S4F_CHECK(rows > 0 && Hq > 0 && Hk > 0, "%s: rows=%lld, Hq=%d, Hk=%d must be positive", who, (long long)rows, Hq, Hk);
-  S4F_CHECK(rows * ((int64_t)Hq + Hk) < (1LL << 31) - (1 << 22), "%s: rows x heads must stay below 2^31 - 2^22", who);
+  S4F_CHECK(rows < (1LL << 31) && rows * ((int64_t)Hq + Hk) < (1LL << 31) - (1 << 22), "%s: rows x heads must stay below 2^31 - 2^22", who);
   S4F_CHECK((gq != nullptr) == (gk != nullptr) && (cos != nullptr) == (sin != nullptr), "%s: gains and tables come in pairs", who);
   S4F_CHECK(gq || cos, "%s: neither a norm (gains) nor a rotation (tables) asked for", who);
-  S4F_CHECK(!gq || (eps > 0.f && eps <= 1e30f), "%s: eps must be positive and finite", who);
+  // (the hardware's reciprocal root takes a denormal argument for zero: a row of zeros would become 0 x infinity)
+  S4F_CHECK(!gq || (eps >= FLT_MIN && eps <= 1e30f), "%s: eps must be finite and at least the least normal fp32 number", who);
   S4F_CHECK(!cos || (period > 0 && period <= rows && rows % period == 0), "%s: the tables' %lld positions must divide the %lld rows", who,
             (long long)period, (long long)rows);
   for (const void* p : {(const void*)gq, (const void*)gk, (const void*)cos, (const void*)sin})
@@ -300,6 +302,8 @@ S4F_API int s4f_qk_norm_rope_fwd(const void* x, int64_t ldx, void* y, int64_t ld
   if (int rc = check_rows(who, "x", x, ldx, dtype)) return rc;
   if (int rc = check_rows(who, "y", y, ldy, dtype)) return rc;
   S4F_CHECK(rows == 1 || ldy >= (int64_t)(Hq + Hk) * 64, "%s: rows of y overlap", who);
+  // (a launch has at most 2^32 - 1 threads; a head takes 4 or 8 of them.  128 GiB of T)
+  S4F_CHECK(rows * (Hq + Hk) <= (dtype == S4F_BF16 ? 1LL << 30 : 1LL << 29) - 64, "%s: rows x heads too large for one launch", who);
   S4F_CHECK((codes != nullptr) == (scales != nullptr) && (!codes || gq), "%s: a checkpoint needs codes, scales and the norm", who);
   S4F_CHECK((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 2 == 0, "%s: codes / scales alignment (16 / 2 bytes)", who);
   QkArgs a{};
@@ -311,8 +315,8 @@ S4F_API int s4f_qk_norm_rope_fwd(const void* x, int64_t ldx, void* y, int64_t ld
 }
 
 int64_t s4f_qk_ws_bytes(int64_t rows, int Hq, int Hk) {
-  if (rows <= 0 || Hq <= 0 || Hk <= 0) return -1;
-  return ((int64_t)bwd_blocks(rows, Hq, Hq + Hk, 32) + bwd_blocks(rows, Hk, Hq + Hk, 32)) * 64 * 4;
+  if (rows <= 0 || rows >= (1LL << 31) || Hq <= 0 || Hk <= 0) return -1;
+  return ((int64_t)bwd_blocks(rows, Hq, (int64_t)Hq + Hk, 32) + bwd_blocks(rows, Hk, (int64_t)Hq + Hk, 32)) * 64 * 4;
 }
 
 S4F_API int s4f_qk_norm_rope_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int8_t* codes, const uint8_t* scales,

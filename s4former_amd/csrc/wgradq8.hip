@@ -347,7 +347,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args 
 
   // ---- sums: to the slab in the order of the registers (16 bytes a lane, whole lines), or to their places
   if (P.splits > 1) {
-f32x4* s = reinterpret_cast<f32x4*>(P.slab) + ((int64_t)(z * P.tiles + tile) * (TM * TN / 4)) + wave * (MI * NI * 4 * 64) + l;
+    f32x4* s = reinterpret_cast<f32x4*>(P.slab) + ((int64_t)(z * P.tiles + tile) * (TM * TN / 4)) + wave * (MI * NI * 4 * 64) + l;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -507,7 +507,7 @@ int64_t s4f_wgrad_packed_ws(const int64_t* dims, int ndims) {
   a.count = (ndims - 1) / 3;
   for (int i = 0; i < a.count; ++i) {
     const int64_t* d = dims + 1 + 3 * i;
-    if (d[0] > INT32_MAX || d[1] > INT32_MAX) return -1;
+    if (d[0] <= 0 || d[0] > INT32_MAX || d[1] <= 0 || d[1] > INT32_MAX) return -1;
     a.p[i].M = (int)d[0]; a.p[i].N = (int)d[1]; a.p[i].rows = d[2];
   }
   return plan(a, (int)dims[0]);

@@ -26,6 +26,8 @@ BWD = dict(dy=P, lddy=128, x=P, ldx=128, codes=None, scales=None, dx=P, lddx=128
     (dict(dtype=2), 'dtype'), (dict(rows=0), 'positive'), (dict(Hq=0), 'positive'), (dict(Hk=-1), 'positive'),
     (dict(rows=1 << 31, period=1 << 31), '2^31'), (dict(gk=None), 'pairs'), (dict(sin=None), 'pairs'),
     (dict(gq=None, gk=None, cos=None, sin=None), 'neither'), (dict(eps=0.0), 'eps'), (dict(eps=float('nan')), 'eps'), (dict(eps=float('inf')), 'eps'),
+    (dict(eps=1e-39), 'eps'), (dict(rows=1 << 61, period=4, Hq=4, Hk=4, ldx=512, ldy=512), '2^31'), (dict(rows=1 << 29), 'one launch'),
+    (dict(rows=(1 << 28), dtype=0), 'one launch'),
     (dict(period=3), 'divide'), (dict(period=0), 'divide'), (dict(period=16), 'divide'), (dict(x=None), 'null'), (dict(y=None), 'null'),
     (dict(x=P + 2), '16-byte'), (dict(ldx=129), '16-byte'), (dict(ldy=130), '16-byte'), (dict(ldy=120), 'overlap'), (dict(gq=P + 4), 'aligned'),
     (dict(cos=P + 8), 'aligned'), (dict(codes=P), 'checkpoint'), (dict(scales=P), 'checkpoint'), (dict(codes=P + 8, scales=P), 'alignment'),
@@ -51,7 +53,7 @@ PACK = dict(x=P, ldx=64, codes=P, scales=P, rows=4, C=64, dtype=1, stream=None)
 @pytest.mark.parametrize('change,match', [
     (dict(dtype=7), 'dtype'), (dict(x=None), 'null'), (dict(codes=None), 'null'), (dict(scales=None), 'null'), (dict(rows=0), 'positive'),
     (dict(C=0), '32'), (dict(C=48), '32'), (dict(C=-32), '32'), (dict(x=P + 2), '16-byte'), (dict(ldx=68), '16-byte'), (dict(ldx=-64), '16-byte'),
-    (dict(codes=P + 4), '16-byte'), (dict(rows=1 << 50), 'too large'), (dict(ldx=128, rows=1 << 31), 'too large'),
+    (dict(codes=P + 4), '16-byte'), (dict(rows=1 << 50), 'too large'), (dict(rows=1 << 31), 'too large'), (dict(ldx=128, rows=1 << 31), 'too large'),
 ])
 def test_pack_entries_refuse(change, match):
     a = {**PACK, **change}
@@ -96,6 +98,11 @@ def test_workspace_queries():
             K.wgrad_packed_ws_bytes(bad, 1)
     with pytest.raises(S4FError):
         K.workspace_bytes(K.WS_QK_NORM, 4, 0, 1)
+    for bad in ((1 << 61, 4, 4), (4, (5 - (1 << 32)), 1), (4, 1, 1 << 32)):
+        with pytest.raises(S4FError):
+            K.workspace_bytes(K.WS_QK_NORM, *bad)
+    with pytest.raises(S4FError):
+        K.wgrad_packed_ws_bytes([(8 - (1 << 32), 32, 5)], 1)
 
 
 def test_front_refuses():
