@@ -34,12 +34,29 @@ __device__ __forceinline__ int work_of_block(int total) {
 }
 
 // ------------------------------------------------------------------------------------------------- fp32
-// 64 x 64 tile, four waves of 32 x 32, 64 rows a step, two buffers, two tiles a CU.  The fp32 matrix rate (256 operations a clock and CU)
-// bounds large problems; the small tile keeps ragged sizes from wasting it, the long step covers the latency of the next one's loads.
-constexpr int BT = 64, BKR = 64, LDF = BT * 4 + 16;      // bytes of a row in LDS: rows 4 apart lie 16 banks apart
+// 64 x 64 tile, four waves with one product of 32 x 32 x 2 each, 64 rows a step, two buffers, two tiles a CU.  The fp32 matrix rate (256
+// operations a clock and CU: 2,048 clocks a step) bounds large problems; the small tile keeps ragged sizes from wasting it.  Counters say
+// that a SIMD issues no other vector instruction beside an fp32 product: 2,760 clocks a step with one block on a CU, 2,480 for each of
+// two.  Measured: 768 x 768 over 16,400 rows 164 us (118 TFLOP/s), 520 x 416 over 2,307 rows 19 us with the join.
+//
+// LDS image: [16 groups of four rows][64 columns], a column's four rows in 16 bytes: a thread turns the 4 x 4 block that it loaded in
+// its registers, and one 16-byte read a lane feeds four products.  Bits 3 and 4 of a column move its lower two, so that the
+// stores, whose lanes are four columns apart, touch different banks (no conflicts are counted).
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+// everyone's accesses of LDS are done (loads that go there among them), those of registers need not be
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+constexpr int BT = 64, BKR = 64;
+__device__ __forceinline__ int f32_place(int col) { return col ^ (col >> 3 & 3); }
 
-__global__ __launch_bounds__(256) void wgrad_f32_kernel(const Args args) {
-  __shared__ __attribute__((aligned(16))) char la[2][BKR * LDF], lb[2][BKR * LDF];      // 68 KiB
+__global__ __launch_bounds__(256, 2) void wgrad_f32_kernel(const Args args) {
+  __shared__ u32x4 la[2][BKR / 4 * BT];
+  __shared__ f32x4 lb[2][BKR / 4 * BT];                   // 64 KiB in all
   const int w = work_of_block(args.p[args.count - 1].work_end);
   int which = 0;
   for (int i = 0; i < MAXP - 1; ++i) which += i < args.count - 1 && w >= args.p[i].work_end ? 1 : 0;
@@ -48,94 +65,116 @@ __global__ __launch_bounds__(256) void wgrad_f32_kernel(const Args args) {
   const int z = local / P.tiles, tile = local - z * P.tiles;
   const int m0 = tile / P.tiles_n * BT, n0 = tile % P.tiles_n * BT;
   const int k_beg = z * P.steps_per_split, k_end = min(k_beg + P.steps_per_split, P.steps);
-  const int N = P.N, M = P.M;
+  const int N = P.N, M = P.M, ns = N / ACTQ8_GROUP;
 
-  const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, g = l >> 4, li = l & 15;
-  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-  // a thread's chunks: rows tid / 16 (+ 16 ..) of dY, four values; rows tid / 8 and + 32 of the codes, eight values (M is a multiple of 8
-  // and N of 32: a chunk is inside or outside)
-  const int ra = tid >> 4, ca = (tid & 15) * 4, rb = tid >> 3, cb = (tid & 7) * 8;
-  const bool aok = m0 + ca < M, bok = n0 + cb < N;
-  const float* pa = reinterpret_cast<const float*>(P.dy) + ((int64_t)k_beg * BKR + ra) * P.lddy + m0 + ca;
-  const int8_t* pb = P.codes + ((int64_t)k_beg * BKR + rb) * N + n0 + cb;
-  const uint8_t* ps = P.scales + ((int64_t)k_beg * BKR + rb) * (N / ACTQ8_GROUP) + (n0 + cb) / ACTQ8_GROUP;
-  int64_t left = P.rows - (int64_t)k_beg * BKR;            // rows from the step on
-
-  constexpr int NA = BKR / 16, NB = BKR / 32;
-  chunk16 xa[NA];
-  uint2 xb[NB];
-  uint32_t xs[NB];
-  auto load = [&]() {
-#pragma unroll
-    for (int i = 0; i < NA; ++i) xa[i] = aok && ra + 16 * i < left ? ld_global16(pa + (int64_t)(16 * i) * P.lddy) : zero16();
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const bool ok = bok && rb + 32 * i < left;
-      xb[i] = ok ? *reinterpret_cast<const uint2*>(pb + (int64_t)(32 * i) * N) : make_uint2(0, 0);
-      xs[i] = ok ? ps[(int64_t)(32 * i) * (N / ACTQ8_GROUP)] : 0u;
-    }
-    pa += (int64_t)BKR * P.lddy; pb += (int64_t)BKR * N; ps += (int64_t)BKR * (N / ACTQ8_GROUP); left -= BKR;
+  const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
+  const int wm = (wave >> 1) * 32 + (l & 31), wn = (wave & 1) * 32 + (l & 31);
+  // a thread's block: rows 4 rg .. + 3, columns c4 .. + 3 of dY and of the codes (M is a multiple of 8 and N of 32: inside or outside).  The
+  // resources cover the rows of the step, so rows behind the range read as zero; columns outside get an offset beyond every resource
+  const int rg = tid >> 4, c4 = (tid & 15) * 4;
+  const int OUT = (int)0x80000000;
+  const int ld4 = (int)(P.lddy * 4);
+  const int va = m0 + c4 < M ? 4 * rg * ld4 + (m0 + c4) * 4 : OUT;
+  const int vb = n0 + c4 < N ? 4 * rg * N + n0 + c4 : OUT;
+  const int vs = n0 + c4 < N ? 4 * rg * ns + (n0 + c4) / ACTQ8_GROUP : OUT;
+  const int64_t r_beg = (int64_t)k_beg * BKR;
+  int left = (int)(min(P.rows, (int64_t)k_end * BKR) - r_beg);
+  char* pa = (char*)P.dy + r_beg * ld4;
+  char* pb = (char*)P.codes + r_beg * N;
+  char* ps = (char*)P.scales + r_beg * ns;
+  __amdgpu_buffer_rsrc_t qa, qb, qs;
+  auto next_rows = [&]() {                                 // the resources of the next step's rows (none left: empty ones)
+    const int nr = __builtin_amdgcn_readfirstlane(max(min(left, BKR), 0));
+    qa = __builtin_amdgcn_make_buffer_rsrc(pa, 0, nr * ld4, 0x00020000);
+    qb = __builtin_amdgcn_make_buffer_rsrc(pb, 0, nr * N, 0x00020000);
+    qs = __builtin_amdgcn_make_buffer_rsrc(ps, 0, nr * ns, 0x00020000);
+    left -= BKR;
+    pa += (int64_t)BKR * ld4; pb += (int64_t)BKR * N; ps += (int64_t)BKR * ns;
   };
-  auto store = [&](int buf) {
+  struct Regs { u32x4 a[4]; uint32_t b[4], s[4]; } R[2];
+  auto load = [&](Regs& r, int i) {                        // row i of the thread's block
+    r.a[i] = __builtin_amdgcn_raw_buffer_load_b128(qa, va + i * ld4, 0, 0);
+    r.b[i] = __builtin_amdgcn_raw_buffer_load_b32(qb, vb + i * N, 0, 0);
+    r.s[i] = __builtin_amdgcn_raw_buffer_load_b8(qs, vs + i * ns, 0, 0);
+  };
+  auto load_all = [&](Regs& r) {
+    next_rows();
 #pragma unroll
-    for (int i = 0; i < NA; ++i) *reinterpret_cast<chunk16*>(la[buf] + (ra + 16 * i) * LDF + ca * 4) = xa[i];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const float s = q8_scale(xs[i]);
-      f32x4 v0, v1;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) { v0[e] = q8_code(xb[i].x, e) * s; v1[e] = q8_code(xb[i].y, e) * s; }
-      *reinterpret_cast<f32x4*>(lb[buf] + (rb + 32 * i) * LDF + cb * 4) = v0;
-      *reinterpret_cast<f32x4*>(lb[buf] + (rb + 32 * i) * LDF + cb * 4 + 16) = v1;
+    for (int i = 0; i < 4; ++i) {
+      load(r, i);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
+  auto store_a = [&](const Regs& r, int e, int buf) {      // column e of it
+    la[buf][rg * BT + f32_place(c4 + e)] = u32x4{r.a[0][e], r.a[1][e], r.a[2][e], r.a[3][e]};
+  };
+  auto store_b = [&](const Regs& r, int e, int buf) {
+    lb[buf][rg * BT + f32_place(c4 + e)] = f32x4{q8_code(r.b[0], e) * q8_scale(r.s[0]), q8_code(r.b[1], e) * q8_scale(r.s[1]),
+                                                 q8_code(r.b[2], e) * q8_scale(r.s[2]), q8_code(r.b[3], e) * q8_scale(r.s[3])};
+  };
 
-  f32x4 acc[2][2];
+  f32x16 acc;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  const int fa = (l >> 5) * BT + f32_place(wm), fb = (l >> 5) * BT + f32_place(wn);
+  f32x4 A[2] = {}, B[2] = {};                              // fragments of eight rows: the lower half of the wave the first four
+  // eight parts: products of eight rows, reads of the next eight; the first four parts also store the next step's rows, which have
+  // waited in registers for a step, the last four load what takes their place (two steps on).  The order is the one written: a product, then what the matrix unit's 64 cycles leave room for
+  auto step = [&](auto bufc) {
+    constexpr int buf = decltype(bufc)::value;
+    Regs& r = R[buf ^ 1];
+    lds_barrier();
+    next_rows();
+    static_for<BKR / 8>([&](auto tc) {
+      constexpr int t = decltype(tc)::value, cur = (t + 1) & 1, nxt = t & 1;
+      static_for<4>([&](auto ec) {
+        constexpr int e = decltype(ec)::value;
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(A[cur][e], B[cur][e], acc, 0, 0, 0);
+        if constexpr (e == 0) { A[nxt] = __builtin_bit_cast(f32x4, la[buf][fa + 2 * t * BT]); B[nxt] = lb[buf][fb + 2 * t * BT]; }
+        if constexpr (e == 1 && t < 4) store_a(r, t, buf ^ 1);
+        if constexpr (e == 2 && t < 4) store_b(r, t, buf ^ 1);
+        if constexpr (e == 2 && t >= 4) load(r, t - 4);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    });
+  };
+  if (k_beg < k_end) {
+    load_all(R[0]);
+    load_all(R[1]);
+    __builtin_amdgcn_sched_barrier(0);                    // (the counted waits of the loop need R[1]'s loads in front of R[0]'s next ones)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (k_beg < k_end) { load(); store(0); }
-  for (int k = k_beg; k < k_end; ++k) {
-    const int buf = (k - k_beg) & 1;
-    if (k + 1 < k_end) load();
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < BKR; h += 32) {
-      Frag<float> a[2], b[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        lds_read_tr(a[i], la[buf], LDF, h, wm + i * 16);
-        lds_read_tr(b[i], lb[buf], LDF, h, wn + i * 16);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mma16(a[i], b[j], acc[i][j]);
+    for (int e = 0; e < 4; ++e) { store_a(R[0], e, 0); store_b(R[0], e, 0); }
+    load_all(R[0]);
+    int k = k_beg + 1;
+    for (; k < k_end; k += 2) {
+      step(std::integral_constant<int, 0>{});
+      step(std::integral_constant<int, 1>{});
     }
-    if (k + 1 < k_end) store(buf ^ 1);                     // (last read in the step before: everyone has passed the barrier since)
+    if (k == k_end) step(std::integral_constant<int, 0>{});
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(A[1][e], B[1][e], acc, 0, 0, 0);
   }
 
   const bool add = P.splits == 1 && args.accumulate;
-  float* o = P.splits == 1 ? P.out : P.slab + (int64_t)z * M * N;
+  const int n = n0 + wn;
+  if (n >= N) return;
+  float* o = (P.splits == 1 ? P.out : P.slab + (int64_t)z * M * N) + n;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int e = 0; e < 4; ++e) {
+    const int m = m0 + (wave >> 1) * 32 + 8 * e + 4 * (l >> 5);
+    if (m >= M) continue;                                  // (M is a multiple of 8)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int n = n0 + wn + j * 16 + li;
-      if (n >= N) continue;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int m = m0 + wm + i * 16 + 4 * g + r;
-        if (m >= M) continue;
-        float* q = o + (int64_t)m * N + n;
-        *q = add ? *q + acc[i][j][r] : acc[i][j][r];
-      }
+    for (int c = 0; c < 4; ++c) {
+      float* q = o + (int64_t)(m + c) * N;
+      *q = add ? *q + acc[4 * e + c] : acc[4 * e + c];
     }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------- bf16
-// Tile (32 MI WM) x (32 NI WN), WM x WN waves with MI x NI products of 32 x 32 x 16 each; 64 rows of dY and X a step, two buffers in LDS.
+// Tile (32 MI WM) x (32 NI WN), KG groups of WM x WN waves with MI x NI products of 32 x 32 x 16 each; 64 rows of dY and X a step and group,
+// two buffers in LDS.  The groups take the lower and the upper rows of a step; their sums meet in LDS at the end.  KG = 2 serves the smallest
+// tile, 64 x 64 with one product a wave, whose step is bound by what one wave can issue: 128 rows take 0.47 us, 64 rows with one group 0.31.
 // dY goes to LDS without a stop in registers; codes wait about two steps in registers and become bf16 on their way to LDS.
 //   barrier (step k's buffer is complete, the other one free)
 //   part 0: products of step k - 1's last 16 rows, reads of the fragments of step k's rows 0 .. 15, loads of the dY of step k + 1
@@ -150,12 +189,8 @@ __global__ __launch_bounds__(256) void wgrad_f32_kernel(const Args args) {
 // conflicts are counted.  Not faster: four waves with 128 x 128 each (1.38 us a step: a store blocks the wave that also has to feed the
 // matrix unit), a third buffer of dY, the conversions spread over all four parts; touching dY's lines a step ahead costs 15 %.
 //
-// LDS image: [64 rows][columns] bf16, the 64-byte unit u of row r at u ^ (r & 3): the four rows x 64 bytes that half a wave reads in
-// one transposing read lie in different banks, and so do the stores (served eight lanes at a time).
-typedef __attribute__((ext_vector_type(16))) float f32x16;
-typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
-typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
-constexpr int STEP = 64;
+// LDS image: [rows][columns] bf16, the 64-byte unit u of row r at u ^ (r & 3) (two units a row: u ^ (r >> 1 & 1)): the four rows x 64 bytes
+// that half a wave reads in one transposing read lie in different banks, and so do the stores (served eight lanes at a time).
 
 // four rows of 16 columns, transposed (all lanes of the wave take part)
 __device__ __forceinline__ s16x4 tr_read(const char* p) {
@@ -170,9 +205,12 @@ struct Frag8 {                                            // eight rows of a col
   }
 };
 
-template <int MI, int NI, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args args) {
-  constexpr int NT = 64 * WM * WN, TM = 32 * MI * WM, TN = 32 * NI * WN, RA = TM * 2, RB = TN * 2;
+// what the unit of a row is moved by; the lower two bits of the row decide
+template <int COLS> __device__ __forceinline__ int place(int row) { return COLS >= 128 ? row & 3 : row >> 1 & 1; }
+
+template <int MI, int NI, int WM, int WN, int KG>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void wgrad_bf16_kernel(const Args args) {
+  constexpr int NW = WM * WN * KG, NT = 64 * NW, STEP = 64 * KG, TM = 32 * MI * WM, TN = 32 * NI * WN, RA = TM * 2, RB = TN * 2;
   constexpr int CA = TM / 8, CB = TN / 16;                // 16-byte chunks of a row of dY / of codes
   constexpr int NA = STEP * CA / NT, NB = STEP * CB / NT, DA = NT / CA, DB = NT / CB;      // chunks a thread, rows between them
   // one object a buffer: the compiler then sees that a read of one does not wait for what arrives in another
@@ -189,12 +227,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args 
   const int M = P.M, N = P.N;
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63;
-  const int wm = wave / WN, wn = wave % WN;
+  const int kg = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
 
   // ---- global side: chunk i of a thread is DA (DB) rows below chunk i - 1.  The resources cover the rows of the step, so rows behind
   // the range read as zero; columns outside are given an offset beyond every resource.  16 codes come as two loads of 8: four of each
   // eight lanes take (and store) the upper half first, so that the eight 16-byte stores served at once touch different banks
-  const int ra = tid / CA, ua = (tid % CA >> 2) ^ (ra & 3), ca = 4 * ua + (tid & 3), rb = tid / CB, cb = tid % CB, hb = (tid >> 2) & 1;
+  const int ra = tid / CA, ua = (tid % CA >> 2) ^ place<TM>(ra), ca = 4 * ua + (tid & 3), rb = tid / CB, cb = tid % CB, hb = (tid >> 2) & 1;
   const int OUT = (int)0x80000000;
   const int ld2 = (int)(P.lddy * 2), ns = N / ACTQ8_GROUP;
   const int va = m0 + 8 * ca < M ? ra * ld2 + (m0 + 8 * ca) * 2 : OUT;
@@ -226,7 +264,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args 
   constexpr auto b_from = [](int t) { return t * 2 * NB / 3; };
   // dY goes to LDS without a stop in registers: 64 lanes x 16 bytes in a row, so the unit's place is chosen on the source side
   auto load_a = [&](int i, auto bufc) {
-    char* d = (decltype(bufc)::value ? A1 : A0) + (WM * WN * i + wave) * 1024;
+    char* d = (decltype(bufc)::value ? A1 : A0) + (NW * i + wave) * 1024;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(qa, (__attribute__((address_space(3))) void*)d, 16, va + i * DA * ld2, 0, 0, 0);
   };
   auto load_b = [&](Regs& r, int i) {                     // half chunk i; the chunk's scale behind its second half
@@ -236,7 +274,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args 
 
   // ---- LDS side.  DA and DB are multiples of 4: a thread's rows agree in their lower two bits
   static_assert(DA % 4 == 0 && DB % 4 == 0, "the unit's place depends on the thread alone");
-  const int ob = rb * RB + (((cb >> 1) ^ (rb & 3)) << 6) + (cb & 1) * 32 + 16 * hb, ob2 = ob + 16 - 32 * hb;
+  const int ob = rb * RB + (((cb >> 1) ^ place<TN>(rb)) << 6) + (cb & 1) * 32 + 16 * hb, ob2 = ob + 16 - 32 * hb;
   u32x4 conv;                                             // the half chunk under conversion
   float cs = 0.f;                                         // and its scale
   auto convert = [&](const Regs& r, int i, int e, auto bufc) {                   // two codes of half chunk i; the last two store it
@@ -250,9 +288,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args 
   const int g = l >> 4, q = (l >> 2) & 3, p4 = l & 3;
   int fa[MI], fb[NI];
 #pragma unroll
-  for (int i = 0; i < MI; ++i) fa[i] = (8 * (g >> 1) + q) * RA + (((wm * MI + i) ^ q) << 6) + (g & 1) * 32 + p4 * 8;
+  for (int i = 0; i < MI; ++i) fa[i] = (64 * kg + 8 * (g >> 1) + q) * RA + (((wm * MI + i) ^ place<TM>(q)) << 6) + (g & 1) * 32 + p4 * 8;
 #pragma unroll
-  for (int j = 0; j < NI; ++j) fb[j] = (8 * (g >> 1) + q) * RB + (((wn * NI + j) ^ q) << 6) + (g & 1) * 32 + p4 * 8;
+  for (int j = 0; j < NI; ++j) fb[j] = (64 * kg + 8 * (g >> 1) + q) * RB + (((wn * NI + j) ^ place<TN>(q)) << 6) + (g & 1) * 32 + p4 * 8;
   struct Frags { Frag8 a[MI], b[NI]; } F[2];
   auto read = [&](Frags& f, int i, auto bufc, int part) { // read i of 2 (NI + MI)
     const int row = part * 16 + 4 * (i & 1);
@@ -269,11 +307,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args 
   auto mma = [&](const Frags& f, int i) {
     acc[i / NI][i % NI] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a[i / NI].v(), f.b[i % NI].v(), acc[i / NI][i % NI], 0, 0, 0);
   };
-  auto barrier = [&]() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-  };
   // vector loads of a step behind its loads of dY: the half chunks of shares 1 and 2 and their scales at least
   constexpr int BEHIND = (2 * NB - b_from(1)) + (NB - b_from(1) / 2);
   constexpr int WAIT = (BEHIND & 15) | (BEHIND >> 4 << 14) | (7 << 4) | (15 << 8);       // vmcnt(BEHIND), the other counters free
@@ -284,7 +317,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args 
   // one part: products of f, fragments of (buffer rbuf, part rpart) to n; share T < 3 of r to buffer sbuf, its registers refilled.  The
   // order is the one written here: a product, then what the matrix unit's 32 cycles leave room for
   auto part = [&](const Frags& f, Frags& n, auto rbuf, int rpart, Regs& r, auto tc, auto sbuf) {
-    constexpr int T = decltype(tc)::value, P = MI * NI, RD = 2 * (MI + NI), RP = T < 3 ? P : P / 2;
+    constexpr int T = decltype(tc)::value, P = MI * NI, RD = 2 * (MI + NI), RP = T < 3 || P == 1 ? P : P / 2;
     constexpr int na = T == 0 ? NA : 0, b0 = T < 3 ? b_from(T) : 0, nc = T < 3 ? 4 * (b_from(T + 1) - b0) : 0;
     static_for<P>([&](auto ic) {
       constexpr int i = decltype(ic)::value;
@@ -307,7 +340,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args 
     using Oth = std::integral_constant<int, b ^ 1>;
     Regs& r = R[b ^ 1];
     __builtin_amdgcn_s_waitcnt(WAIT);                     // this wave's dY of the step has arrived (the loads of codes behind it need not have)
-    barrier();
+    lds_barrier();
     next_rows();
     next_rows_a();
     part(F[1], F[0], Cur{}, 0, r, I0{}, Oth{});
@@ -336,13 +369,38 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wgrad_bf16_kernel(const Args 
     for (int i = 0; i < MI; ++i) F[1].a[i] = Frag8{};
 #pragma unroll
     for (int j = 0; j < NI; ++j) F[1].b[j] = Frag8{};
-    for (int k = k_beg; k < k_end; k += 2) {              // (behind the last step of an odd range: one on zeros)
-      step(I0{});
-      step(I1{});
+    if constexpr (KG == 1) {
+      for (int k = k_beg; k < k_end; k += 2) {            // (behind the last step of an odd range: one on zeros)
+        step(I0{});
+        step(I1{});
+      }
+    } else {
+      int k = k_beg + 1;
+      for (; k < k_end; k += 2) {
+        step(I0{});
+        step(I1{});
+      }
+      if (k == k_end) step(I0{});
     }
 #pragma unroll
     for (int i = 0; i < MI * NI; ++i) mma(F[1], i);
     __builtin_amdgcn_s_waitcnt(15 << 8 | 7 << 4);           // nothing arrives in LDS behind the wave's end: vmcnt(0)
+  }
+  if constexpr (KG == 2) {                                // the upper rows' sums join the lower rows'
+    static_assert(MI * NI == 1 && STEP * RA >= 4 * 64 * WM * WN * 16, "a wave's sums fit its share of a buffer");
+    f32x4* s = reinterpret_cast<f32x4*>(A0) + (wave % (WM * WN)) * 256 + l;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (kg == 1) s[e * 64] = f32x4{acc[0][0][4 * e], acc[0][0][4 * e + 1], acc[0][0][4 * e + 2], acc[0][0][4 * e + 3]};
+    __syncthreads();
+    if (kg == 1) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const f32x4 v = s[e * 64];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[0][0][4 * e + c] += v[c];
+    }
   }
 
   // ---- sums: to the slab in the order of the registers (16 bytes a lane, whole lines), or to their places
@@ -418,12 +476,15 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const Args args) {
   }
 }
 
-// Tile variants and the number of row ranges.  Time of a step of 64 rows with one tile on the chip's CUs or fewer (`one`) and with every
-// place taken (`full`: the clock drops with the power that the matrix units draw), measured on 2304 x 768 and 4096 x 4096; a range
-// costs about 3 us to start and end, a join 4 us and 5.5 TB/s for writing and reading the slabs.  The large tile moves the fewest
-// bytes per product, the small ones fill the chip on small outputs with fewer ranges, hence smaller slabs.
-struct Variant { int tm, tn, slots; double one, full; };
-constexpr Variant VAR[3] = {{256, 256, 256, 1.21, 1.65}, {256, 128, 256, 0.76, 0.97}, {128, 128, 512, 0.58, 1.11}};
+// Tile variants and the number of row ranges.  Time of a step with one tile on the chip's CUs or fewer (`one`) and with every place taken
+// (`full`: the clock drops with the power that the matrix units draw; between them in proportion, for the smallest tile at once when two
+// of its blocks share a CU), measured on 2304 x 768, 4096 x 4096 and, the smallest, 768 x 768 and 2304 x 768; a range costs about 3 us to
+// start and end, a join 4 us and 5.5 TB/s for writing and reading the slabs.  Over 34 sets of sizes from 192 x 192 to a layer of 1024 / 4096,
+// 130 to 34,000 rows, each timed with every tile and 16 numbers of ranges, the choice is 1 % off the best on average and 15 % at most.  The large tile moves the fewest bytes per product, the
+// small ones fill the chip on small outputs with fewer ranges, hence smaller slabs: 768 x 768 over 1,025 rows takes 7.8 us with the smallest
+// tile and no range, 12.7 us with 128 x 128 in two.
+struct Variant { int tm, tn, step, slots; double one, full; };
+constexpr Variant VAR[4] = {{256, 256, 64, 256, 1.21, 1.65}, {256, 128, 64, 256, 0.76, 0.97}, {128, 128, 64, 512, 0.58, 1.11}, {64, 64, 128, 512, 0.50, 0.87}};
 
 // sets tiles, row ranges and work of the problems for (tile, at most s ranges); returns the bytes of slabs
 int64_t lay_out(Args& a, int tm, int tn, int step, int s, bool exact_slabs) {
@@ -452,47 +513,65 @@ int64_t plan(Args& a, int dtype) {
     if (p.M <= 0 || p.N <= 0 || p.rows <= 0 || p.M % 8 || p.N % ACTQ8_GROUP || p.rows >= (1LL << 31) - 128 || (int64_t)p.M * p.N > (1LL << 31)) return -1;
   }
   if (dtype == S4F_F32) {
-    // two tiles a CU, four where a range keeps sixteen steps (520 x 416 over 2,307 rows: 24 us with 8 ranges of 5 steps, 28 with 13 of 3;
-    // 768 x 768 over 16,400: 238 us with 3 of 86, 209 with 7 of 37)
+    // as many ranges as give every CU one, two .. twelve blocks, by the time of a step of 64 rows: 1.17 us with one block on a CU, 1.05 for
+    // each of several; start, end, join and slabs as below (520 x 416 over 2,307 rows: 19 us with 4 ranges of 10 steps, 21 with 8 of 5; 768 x 768
+    // over 16,400: 164 us with 7, 186 with 3)
     lay_out(a, BT, BT, BKR, 1, true);
     const int tiles = a.p[a.count - 1].work_end;
-    int steps = 0;
-    for (int i = 0; i < a.count; ++i) steps = std::max(steps, a.p[i].steps);
-    const int64_t bytes = lay_out(a, BT, BT, BKR, std::max(1, std::min(1024 / tiles, std::max(512 / tiles, steps / 16))), true);
+    double best = 0;
+    int bs = 1, last = 0;
+    for (int c = 0; c <= 12; ++c) {
+      const int s = std::max(1, 256 * c / tiles);
+      if (s == last) continue;
+      last = s;
+      int64_t items = 0, slabs = 0;
+      int longest = 0;
+      for (int i = 0; i < a.count; ++i) {
+        const int each = ceil_div(a.p[i].steps, std::max(1, std::min(s, a.p[i].steps / 2))), n = ceil_div(a.p[i].steps, each);
+        longest = std::max(longest, each);
+        items += (int64_t)a.p[i].tiles * n;
+        if (n > 1) slabs += (int64_t)a.p[i].M * a.p[i].N * n;
+      }
+      const int64_t share = (items + 255) / 256;
+      const double t = longest * (share == 1 ? 1.17 : 1.05 * share) + 3 + (slabs ? 4 + 8e-6 / 5.5 * slabs : 0);
+      if (c == 0 || t < best) { best = t; bs = s; }
+    }
+    const int64_t bytes = lay_out(a, BT, BT, BKR, bs, true);
     return a.p[a.count - 1].work_end < INT32_MAX ? bytes : -1;
   }
   double best = 0;
   int bs = 0;
-  for (int v = 0; v < 3; ++v) {
+  for (int v = 0; v < 4; ++v) {
     int64_t tiles[MAXP], all = 0;
     for (int i = 0; i < a.count; ++i) {
       tiles[i] = (int64_t)ceil_div(a.p[i].M, VAR[v].tm) * ceil_div(a.p[i].N, VAR[v].tn);
       all += tiles[i];
     }
-    const int fill = (int)std::min<int64_t>(VAR[v].slots / all, 64);             // ranges that take every place once
-    for (int s : {1, 2, 3, 4, fill / 2, fill}) {
+    const int most = (int)std::min<int64_t>(VAR[v].slots / all, 64);             // ranges that take every place once
+    for (int s : {1, 2, 3, 4, most / 2, most}) {
       if (s < 1) continue;
       int64_t items = 0, slabs = 0;
       int longest = 0;
       for (int i = 0; i < a.count; ++i) {
-        const int steps = ceil_div(a.p[i].rows, STEP), per = ceil_div(steps, std::max(1, std::min(s, steps / 2))), n = ceil_div(steps, per);
-        longest = std::max(longest, per);
+        const int steps = ceil_div(a.p[i].rows, VAR[v].step), each = ceil_div(steps, std::max(1, std::min(s, steps / 2))), n = ceil_div(steps, each);
+        longest = std::max(longest, each);
         items += tiles[i] * n;
         if (n > 1) slabs += tiles[i] * n;
       }
-      const double rest = (double)(items % VAR[v].slots) / VAR[v].slots, per = ((longest + 1) & ~1) + 0.25;
+      const bool small = VAR[v].step == 128;
+      const double rest = (double)(items % VAR[v].slots) / VAR[v].slots, fill = small ? rest > 0.5 : rest, per = (small ? longest : (longest + 1) & ~1) + 0.25;
       const double t = (double)(items / VAR[v].slots) * (per * VAR[v].full + 3) +
-                       (rest > 0 ? per * (VAR[v].one + rest * (VAR[v].full - VAR[v].one)) + 3 : 0) +
+                       (rest > 0 ? per * (VAR[v].one + fill * (VAR[v].full - VAR[v].one)) + 3 : 0) +
                        (slabs ? 4 + 8e-6 / 5.5 * slabs * VAR[v].tm * VAR[v].tn : 0);
       if (bs == 0 || t < best) { best = t; a.variant = v; bs = s; }
     }
   }
-  const int64_t bytes = lay_out(a, VAR[a.variant].tm, VAR[a.variant].tn, STEP, bs, false);
+  const int64_t bytes = lay_out(a, VAR[a.variant].tm, VAR[a.variant].tn, VAR[a.variant].step, bs, false);
   return a.p[a.count - 1].work_end < INT32_MAX ? bytes : -1;
 }
 
-template <int MI, int NI, int WM, int WN> void launch_bf16(const Args& a, hipStream_t st) {
-  hipLaunchKernelGGL((wgrad_bf16_kernel<MI, NI, WM, WN>), dim3(a.p[a.count - 1].work_end), dim3(64 * WM * WN), 0, st, a);
+template <int MI, int NI, int WM, int WN, int KG = 1> void launch_bf16(const Args& a, hipStream_t st) {
+  hipLaunchKernelGGL((wgrad_bf16_kernel<MI, NI, WM, WN, KG>), dim3(a.p[a.count - 1].work_end), dim3(64 * WM * WN * KG), 0, st, a);
   int blocks = 0;
   for (int i = 0; i < a.count; ++i) blocks += a.p[i].splits > 1 ? a.p[i].tiles * WM * WN * MI * NI : 0;
   if (blocks) hipLaunchKernelGGL((wgrad_join_bf16_kernel<MI, NI, WM, WN>), dim3(blocks), dim3(256), 0, st, a);
@@ -529,8 +608,8 @@ S4F_API int s4f_wgrad_packed(const s4f_wgrad_packed_desc* descs, int count, int 
     S4F_CHECK(d.M > 0 && d.N > 0 && d.rows > 0 && d.M % 8 == 0 && d.N % ACTQ8_GROUP == 0,
               "%s: M=%d must be a multiple of 8, N=%d of 32, rows=%lld positive", who, d.M, d.N, (long long)d.rows);
     S4F_CHECK(d.lddy >= d.M, "%s: rows of dy overlap (ld %lld < M %d)", who, (long long)d.lddy, d.M);
-    // (the bf16 kernel addresses 64 rows with 32-bit offsets)
-    S4F_CHECK(d.lddy < (1 << 23) && d.N < (1 << 24) && d.rows < (1LL << 31) - 128, "%s: sizes too large for one launch", who);
+    // (the kernels address the rows of a step, 64 or 128, with offsets below 2^31)
+    S4F_CHECK(d.lddy < (1 << 22) && d.N < (1 << 23) && d.rows < (1LL << 31) - 128, "%s: sizes too large for one launch", who);
     Problem& p = a.p[i];
     p.dy = d.dy; p.lddy = d.lddy; p.codes = d.codes; p.scales = d.scales; p.out = d.out; p.M = d.M; p.N = d.N; p.rows = d.rows;
   }
@@ -549,7 +628,8 @@ S4F_API int s4f_wgrad_packed(const s4f_wgrad_packed_desc* descs, int count, int 
   if (dtype == S4F_BF16) {
     if (a.variant == 0) launch_bf16<4, 2, 2, 4>(a, (hipStream_t)stream);
     else if (a.variant == 1) launch_bf16<2, 2, 4, 2>(a, (hipStream_t)stream);
-    else launch_bf16<2, 2, 2, 2>(a, (hipStream_t)stream);
+    else if (a.variant == 2) launch_bf16<2, 2, 2, 2>(a, (hipStream_t)stream);
+    else launch_bf16<1, 1, 2, 2, 2>(a, (hipStream_t)stream);
     S4F_LAUNCH_CHECK();
     return 0;
   }

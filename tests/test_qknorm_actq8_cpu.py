@@ -72,6 +72,7 @@ WG = dict(dy=P, lddy=64, codes=P, scales=P, out=P, rows=4096, M=64, N=64)
     (dict(dy=None), 'null'), (dict(codes=None), 'null'), (dict(scales=None), 'null'), (dict(out=None), 'null'), (dict(M=12), 'multiple'),
     (dict(N=40), 'multiple'), (dict(M=0), 'multiple'), (dict(rows=0), 'multiple'), (dict(lddy=68), '16-byte'), (dict(dy=P + 8), '16-byte'),
     (dict(out=P + 4), '16-byte'), (dict(lddy=0), 'overlap'), (dict(lddy=-64), 'overlap'), (dict(lddy=56), 'overlap'), (dict(lddy=1 << 23), 'too large'),
+    (dict(lddy=1 << 22), 'too large'), (dict(N=1 << 23), 'too large'),
     (dict(N=1 << 24), 'too large'), (dict(rows=(1 << 31) - 100), 'too large'), (dict(rows=1 << 40), 'too large'), (dict(M=1 << 20, N=1 << 20, lddy=1 << 20), 'too large'), (dict(), 'workspace'),
 ])
 def test_wgrad_entry_refuses(change, match):

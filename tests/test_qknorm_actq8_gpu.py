@@ -367,33 +367,39 @@ def test_wgrad(K, code, rows, shapes, pad):
     assert all(torch.equal(a, b) for a, b in zip(again, fresh))                   # the same bits each time
 
 
-# sizes at which the larger tiles are chosen, ragged at both edges and in the rows: 256 x 256 whole and in ranges, 256 x 128 whole and in
-# ranges, and 128 x 128 in many ranges
-LARGE_CASES = [(65, [(4104, 2080)]), (130, [(776, 3104)] * 3), (8199, [(2056, 2080)]), (8199, [(2056, 2080)] * 2), (130, [(4104, 288)] * 3), (4099, [(3080, 288)]), (2050, [(264, 288)] * 3)]
+# sizes at which each tile is chosen, ragged at both edges and in the rows: 256 x 256 whole and in ranges, 256 x 128 whole and in ranges,
+# 128 x 128 whole and in ranges, 64 x 64 whole and in ranges, with odd and even numbers of its steps of 128 rows
+LARGE_CASES = [(65, [(4104, 2080)]), (130, [(776, 3104)] * 3), (8199, [(2056, 2080)]), (8199, [(2056, 2080)] * 2), (130, [(4104, 288)] * 3), (4099, [(3080, 288)]), (2050, [(264, 288)] * 3),
+               (4099, [(1032, 1056)]), (1100, [(1032, 1056)] * 2), (4099, [(1288, 800)]), (128, [(64, 64)]), (129, [(72, 96)]), (256, [(200, 224)]), (300, [(1032, 1056)]),
+               (641, [(72, 32), (520, 416)]), (1025, [(2312, 800)]), (6001, [(200, 224)] * 2), (8199, [(776, 800)])]
 
 
-@pytest.mark.parametrize('rows,shapes', LARGE_CASES)
-def test_wgrad_tiles(K, rows, shapes):
+# fp32: one step, odd and even numbers of steps, one and several ranges, ragged at both edges and in the rows
+F32_CASES = [(64, [(64, 64)]), (65, [(72, 96)]), (129, [(72, 32), (8, 160)]), (577, [(200, 224)]), (2307, [(520, 416)]), (4099, [(776, 800)]), (1025, [(264, 288)] * 3)]
+
+
+@pytest.mark.parametrize('code,rows,shapes', [(1, *c) for c in LARGE_CASES] + [(0, *c) for c in F32_CASES])
+def test_wgrad_tiles(K, code, rows, shapes):
     gen = torch.Generator(device='cuda').manual_seed(rows)
-    need = K.wgrad_packed_ws_bytes([(m, n, rows) for m, n in shapes], 1)
+    need = K.wgrad_packed_ws_bytes([(m, n, rows) for m, n in shapes], code)
     ws = torch.full((max(4, need // 4),), float('nan'), device='cuda')
     probs, refs = [], []
     for m, n in shapes:
-        dy = torch.randn(rows, m + 8, device='cuda', generator=gen).bfloat16()[:, 8:]
-        x = torch.randn(rows, n, device='cuda', generator=gen).bfloat16()
+        dy = torch.randn(rows, m + 8, device='cuda', generator=gen).to(tdt(code))[:, 8:]
+        x = torch.randn(rows, n, device='cuda', generator=gen).to(tdt(code))
         c, s = torch.empty(rows, n, device='cuda', dtype=torch.int8), torch.empty(rows, n // 32, device='cuda', dtype=torch.uint8)
-        K.act_pack(x, c, s, 1)
+        K.act_pack(x, c, s, code)
         probs.append((dy, c, s, torch.full((m, n), float('nan'), device='cuda')))
         xd = c.double() * torch.exp2(s.double() - 127).repeat_interleave(32, 1)
         dt = dy.double().t().contiguous()
         refs.append((dt @ xd, dt.abs() @ xd.abs()))
-    K.wgrad_packed(probs, 1, ws, accumulate=False)
+    K.wgrad_packed(probs, code, ws, accumulate=False)
     for (dy, c, s, out), (ref, mag) in zip(probs, refs):
         within(out, ref.cpu(), 2 * (rows + 16) * U * mag.cpu(), 'dW')
         # a lost step would still be inside the worst case of thousands of additions; their errors are independent and each at most u of a
         # partial sum, which is below mag: eight times their root mean square
         assert float(((out.double() - ref).abs() / mag).max()) <= 8 * U * rows ** 0.5 + 8 * U
-    K.wgrad_packed(probs, 1, ws)
+    K.wgrad_packed(probs, code, ws)
     for (dy, c, s, out), (ref, mag) in zip(probs, refs):
         within(out, 2 * ref.cpu(), (4 * (rows + 16) * U * mag + 4 * U * ref.abs()).cpu(), 'dW added')
 
