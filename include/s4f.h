@@ -227,7 +227,8 @@ int s4f_act_pack(const void* x, int64_t ldx, int8_t* codes, uint8_t* scales, int
 /* y T [rows, C] (row stride ldy) = code s */
 int s4f_act_unpack(const int8_t* codes, const uint8_t* scales, void* y, int64_t ldy, int64_t rows, int C, int dtype, s4f_stream stream);
 /* Weight gradients from checkpoints, up to four problems at once: out fp32 [M, N] (+)= dy^T x, dy T [rows, M] (row stride lddy),
- * x = the restored [rows, N].  M % 8 == 0, N % 32 == 0, lddy >= M.  bf16: products exact.  Sums fp32 in a fixed order.
+ * x = the restored [rows, N].  M % 8 == 0, N % 32 == 0, M <= lddy < 2^22, N < 2^23, rows < 2^31 - 128, M N <= 2^31.  bf16: products
+ * exact.  Sums fp32 in a fixed order.
  * ws: s4f_workspace_bytes(S4F_WS_WGRAD_PACKED, {dtype, M, N, rows, ... of each problem}). */
 typedef struct s4f_wgrad_packed_desc {
   const void* dy; int64_t lddy;
