@@ -7,13 +7,15 @@
 //   dg = sum dz u  (over rows and the heads of the kind),  dx = r (dz g - u mean(dz g u))
 // Everything between the loads and the one rounding of the store is fp32.
 //
-// Layout: LANES lanes (4 for bf16, 8 for fp32) hold a head; a lane has 16 bytes of the lower and 16 bytes of the upper half, so that
-// a rotation's pair stays in the lane, the mean takes two or three lane exchanges, and one 8-bit group (32 channels: a half) is
-// spread over the same lanes.  Both passes are bound by HBM; the tables (256 bytes a row) are read per head but come from cache,
-// the heads of a row being neighbours in the grid.
+// Layout: LANES lanes hold a head; a lane has V = 32 / LANES values of the lower and V of the upper half, so that a rotation's pair stays in
+// the lane, the mean takes two or three lane exchanges, and one 8-bit group (32 channels: a half) is spread over the same lanes.  Four
+// lanes and 16-byte accesses for bf16, eight for fp32; eight also for the backward from x, whose registers then leave room for twice the
+// waves (3 x 2,305 rows, 16 + 4 heads: 14.3 us, with four lanes 15.6; from the checkpoint four are faster by 2 us at 16,400 rows x 24).
+// Both passes are bound by HBM; the tables (256 bytes a row) are read per head but come from cache, the heads of a row being
+// neighbours in the grid.
 //
 // Measured, bf16, 16,400 rows x 24 heads: forward 17.4 us with the tensors in the last-level cache (6.0 TB/s) and 23.3 us on fresh ones
-// (4.5 TB/s; a large copy reaches 4.8 - 5.0), with the checkpoint 21.9 us; backward 25.7 us from the checkpoint and 27.7 us from x,
+// (4.5 TB/s; a large copy reaches 4.8 - 5.0), with the checkpoint 21.9 us; backward 25.7 us from the checkpoint and 27.8 us from x,
 // 4 us of them the join of the gains.  A call on few rows takes 2.5 - 3.5 us on the GPU, less than its launch costs the host.
 #include "actq8.h"
 #include "../../include/s4f.h"
@@ -35,23 +37,18 @@ struct QkArgs {
   int bq;                               // backward: blocks that take query heads (the others take key heads)
 };
 
-template <typename T> __device__ __forceinline__ void unpack16(const chunk16& c, float (&v)[16 / sizeof(T)]);
-template <> __device__ __forceinline__ void unpack16<float>(const chunk16& c, float (&v)[4]) {
+// V values of a lane in one access of 8 or 16 bytes
+template <typename T, int V> struct __attribute__((aligned(V * sizeof(T)))) Vals { T t[V]; };
+template <int V, typename T> __device__ __forceinline__ Vals<T, V> ld_vals(const T* p) { return *reinterpret_cast<const Vals<T, V>*>(p); }
+template <typename T, int V> __device__ __forceinline__ void unpack(const Vals<T, V>& c, float (&v)[V]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(c.w[i]);
+  for (int i = 0; i < V; ++i) v[i] = (float)c.t[i];
 }
-template <> __device__ __forceinline__ void unpack16<bf16_t>(const chunk16& c, float (&v)[8]) {
+template <typename T, int V> __device__ __forceinline__ void st_vals(T* p, const float (&v)[V]) {
+  Vals<T, V> c;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(c.w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(c.w[i] & 0xffff0000u);
-  }
-}
-template <typename T> __device__ __forceinline__ chunk16 pack16(const float (&v)[16 / sizeof(T)]) {
-  union { chunk16 c; T t[16 / sizeof(T)]; } u;
-#pragma unroll
-  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) u.t[i] = from_f32<T>(v[i]);
-  return u.c;
+  for (int i = 0; i < V; ++i) c.t[i] = from_f32<T>(v[i]);
+  *reinterpret_cast<Vals<T, V>*>(p) = c;
 }
 template <int V> struct __attribute__((aligned(V))) Codes { uint32_t w[V / 4]; };           // V codes of a lane
 template <int V> __device__ __forceinline__ void ld_f32(const float* p, float (&v)[V]) {
@@ -64,8 +61,7 @@ template <int V> __device__ __forceinline__ void ld_f32(const float* p, float (&
 
 // r of a head whose lanes hold partial sums of squares.  fp32 operands: correctly rounded root and quotient; bf16: the hardware's
 // reciprocal root (1 ulp of fp32, 2^-15 of a bf16 step)
-template <typename T> __device__ __forceinline__ float inv_rms(float sq, float eps) {
-  constexpr int LANES = 32 / (16 / sizeof(T));
+template <typename T, int LANES> __device__ __forceinline__ float inv_rms(float sq, float eps) {
   const float m = fmaf(group_sum<LANES>(sq), 1.f / 64.f, eps);
   if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rsqf(m);
   return 1.f / sqrtf(m);
@@ -81,8 +77,8 @@ __global__ __launch_bounds__(256) void qk_fwd_kernel(const QkArgs a) {
   const int h = (int)(it - row * (uint32_t)a.H);
   const T* xp = reinterpret_cast<const T*>(a.x) + (int64_t)row * a.ldx + h * 64 + l * V;
   float lo[V], hi[V];
-  unpack16<T>(ld_global16(xp), lo);
-  unpack16<T>(ld_global16(xp + 32), hi);
+  unpack(ld_vals<V>(xp), lo);
+  unpack(ld_vals<V>(xp + 32), hi);
   if constexpr (PACK) {
     uint32_t ml = 0, mh = 0;
 #pragma unroll
@@ -104,7 +100,7 @@ __global__ __launch_bounds__(256) void qk_fwd_kernel(const QkArgs a) {
     float sq = 0.f;
 #pragma unroll
     for (int e = 0; e < V; ++e) sq = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], sq));
-    const float r = inv_rms<T>(sq, a.eps);
+    const float r = inv_rms<T, LANES>(sq, a.eps);
     const float* g = (h < a.Hq ? a.gq : a.gk) + l * V;
     float gl[V], gh[V];
     ld_f32<V>(g, gl);
@@ -125,15 +121,15 @@ __global__ __launch_bounds__(256) void qk_fwd_kernel(const QkArgs a) {
     }
   }
   T* yp = reinterpret_cast<T*>(a.y) + (int64_t)row * a.ldy + h * 64 + l * V;
-  *reinterpret_cast<chunk16*>(yp) = pack16<T>(lo);
-  *reinterpret_cast<chunk16*>(yp + 32) = pack16<T>(hi);
+  st_vals<T, V>(yp, lo);
+  st_vals<T, V>(yp + 32, hi);
 }
 
 // Backward.  A block takes heads of one kind (so that a lane's 2 V gain gradients stay in registers over all its heads) and leaves
 // one row of 64 partial sums; qk_gain_kernel joins them in the order of the blocks: the result does not depend on timing.
 template <typename T, bool NORM, bool ROPE, bool PACK>
 __global__ __launch_bounds__(256) void qk_bwd_kernel(const QkArgs a) {
-  constexpr int V = 16 / sizeof(T), LANES = 32 / V, PER = 256 / LANES;
+  constexpr int V = PACK ? 16 / sizeof(T) : 4, LANES = 32 / V, PER = 256 / LANES;
   const int l = threadIdx.x & (LANES - 1);
   const bool key = (int)blockIdx.x >= a.bq;
   const uint32_t nh = (uint32_t)(key ? a.H - a.Hq : a.Hq), h0 = (uint32_t)(key ? a.Hq : 0);
@@ -152,11 +148,11 @@ __global__ __launch_bounds__(256) void qk_bwd_kernel(const QkArgs a) {
     const uint32_t h = h0 + (it - row * nh);
     const T* dp = reinterpret_cast<const T*>(a.dy) + (int64_t)row * a.lddy + h * 64 + l * V;
     float lo[V], hi[V], xl[V], xh[V];
-    const chunk16 d0 = ld_global16(dp), d1 = ld_global16(dp + 32);
+    const Vals<T, V> d0 = ld_vals<V>(dp), d1 = ld_vals<V>(dp + 32);
     if constexpr (NORM && !PACK) {
       const T* xp = reinterpret_cast<const T*>(a.x) + (int64_t)row * a.ldx + h * 64 + l * V;
-      unpack16<T>(ld_global16(xp), xl);
-      unpack16<T>(ld_global16(xp + 32), xh);
+      unpack(ld_vals<V>(xp), xl);
+      unpack(ld_vals<V>(xp + 32), xh);
     } else if constexpr (NORM) {
       const int64_t hd = (int64_t)row * a.H + h;
       const int8_t* cp = a.codes + hd * 64 + l * V;
@@ -166,8 +162,8 @@ __global__ __launch_bounds__(256) void qk_bwd_kernel(const QkArgs a) {
 #pragma unroll
       for (int e = 0; e < V; ++e) { xl[e] = q8_code(wl.w[e / 4], e & 3) * sl; xh[e] = q8_code(wh.w[e / 4], e & 3) * sh; }
     }
-    unpack16<T>(d0, lo);
-    unpack16<T>(d1, hi);
+    unpack(d0, lo);
+    unpack(d1, hi);
     if constexpr (ROPE) {
       const int64_t t = (int64_t)(row % a.period) * 32 + l * V;
       float c[V], s[V];
@@ -184,7 +180,7 @@ __global__ __launch_bounds__(256) void qk_bwd_kernel(const QkArgs a) {
       float sq = 0.f, dot = 0.f;
 #pragma unroll
       for (int e = 0; e < V; ++e) sq = fmaf(xl[e], xl[e], fmaf(xh[e], xh[e], sq));
-      const float r = inv_rms<T>(sq, a.eps);
+      const float r = inv_rms<T, LANES>(sq, a.eps);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         xl[e] *= r; xh[e] *= r;                            // u
@@ -198,8 +194,8 @@ __global__ __launch_bounds__(256) void qk_bwd_kernel(const QkArgs a) {
       for (int e = 0; e < V; ++e) { lo[e] = r * fmaf(-xl[e], m, lo[e]); hi[e] = r * fmaf(-xh[e], m, hi[e]); }
     }
     T* yp = reinterpret_cast<T*>(a.y) + (int64_t)row * a.ldy + h * 64 + l * V;
-    *reinterpret_cast<chunk16*>(yp) = pack16<T>(lo);
-    *reinterpret_cast<chunk16*>(yp + 32) = pack16<T>(hi);
+    st_vals<T, V>(yp, lo);
+    st_vals<T, V>(yp + 32, hi);
   }
   if constexpr (NORM) {
     __shared__ float sum[4][64];
@@ -244,11 +240,13 @@ __global__ __launch_bounds__(256) void qk_gain_kernel(const float* __restrict__ 
   }
 }
 
-// blocks of the backward for the heads of one kind: 1,024 in all at most, in proportion, each with at least one full turn of its lanes.
-// (Measured at 16,400 rows x 24 heads, bf16: 512 a kind 25.8 us, 384 26.3, 1,024 26.8, 2,048 30.2: the blocks end with a reduction and
-// leave 256 bytes each to be joined.)
-int bwd_blocks(int64_t rows, int64_t heads, int64_t all, int per) {
-  const int64_t b = (rows * heads + per - 1) / per, cap = std::max<int64_t>(1, (int64_t)1024 * heads / all);
+// heads that a block of the backward takes at a time, and blocks for the heads of one kind: `most` in all at most, in proportion, each with
+// at least one full turn of its lanes.  (Measured in bf16, 16,400 rows x 24 heads from the checkpoint: 1,024 blocks 25.8 us, 768 26.3, 2,048
+// 26.8, 4,096 30.2; from x 768 27.8 us, 1,024 28.4, 512 28.2, 2,048 28.7: the blocks end with a reduction and leave 256 bytes each to be joined.)
+int bwd_heads(bool packed, int dtype) { return packed && dtype == S4F_BF16 ? 64 : 32; }
+int bwd_most(bool packed) { return packed ? 1024 : 768; }
+int bwd_blocks(int64_t rows, int64_t heads, int64_t all, int per, int most) {
+  const int64_t b = (rows * heads + per - 1) / per, cap = std::max<int64_t>(1, most * heads / all);
   return (int)std::min(b, cap);
 }
 
@@ -316,7 +314,7 @@ S4F_API int s4f_qk_norm_rope_fwd(const void* x, int64_t ldx, void* y, int64_t ld
 
 int64_t s4f_qk_ws_bytes(int64_t rows, int Hq, int Hk) {
   if (rows <= 0 || rows >= (1LL << 31) || Hq <= 0 || Hk <= 0) return -1;
-  return ((int64_t)bwd_blocks(rows, Hq, (int64_t)Hq + Hk, 32) + bwd_blocks(rows, Hk, (int64_t)Hq + Hk, 32)) * 64 * 4;
+  return ((int64_t)bwd_blocks(rows, Hq, (int64_t)Hq + Hk, 32, 1024) + bwd_blocks(rows, Hk, (int64_t)Hq + Hk, 32, 1024)) * 64 * 4;
 }
 
 S4F_API int s4f_qk_norm_rope_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int8_t* codes, const uint8_t* scales,
@@ -341,9 +339,9 @@ S4F_API int s4f_qk_norm_rope_bwd(const void* dy, int64_t lddy, const void* x, in
   a.dy = dy; a.lddy = lddy; a.x = x; a.ldx = ldx; a.y = dx; a.ldy = lddx; a.gq = gq; a.gk = gk; a.cos = cos; a.sin = sin;
   a.codes = gq ? const_cast<int8_t*>(codes) : nullptr; a.scales = const_cast<uint8_t*>(scales); a.part = (float*)ws; a.eps = eps;
   a.rows = (uint32_t)rows; a.period = (uint32_t)(cos ? period : 1); a.Hq = Hq; a.H = Hq + Hk;
-  const int per = dtype == S4F_BF16 ? 64 : 32;
-  a.bq = bwd_blocks(rows, Hq, Hq + Hk, per);
-  const int blocks = a.bq + bwd_blocks(rows, Hk, Hq + Hk, per);
+  const int per = bwd_heads(a.codes, dtype), most = bwd_most(a.codes);
+  a.bq = bwd_blocks(rows, Hq, Hq + Hk, per, most);
+  const int blocks = a.bq + bwd_blocks(rows, Hk, Hq + Hk, per, most);
   if (dtype == S4F_BF16) launch_bwd<bf16_t>(a, blocks, (hipStream_t)stream); else launch_bwd<float>(a, blocks, (hipStream_t)stream);
   S4F_LAUNCH_CHECK();
   if (gq) {
