@@ -11,8 +11,21 @@
 // stands for zeros.
 #pragma once
 #include "common.h"
+#include <initializer_list>
 
 #define ACTQ8_GROUP 32
+
+// host side of the argument checks: a piece of memory, and whether two have a byte in common
+struct Piece { const char* p; int64_t n; };
+inline Piece piece(const void* p, int64_t n) { return {(const char*)p, p ? n : 0}; }
+// [rows, cols] with a row stride of ld elements of es bytes, from its first byte to its last
+inline Piece piece(const void* p, int64_t rows, int64_t ld, int64_t cols, int es) { return piece(p, ((rows - 1) * ld + cols) * es); }
+inline bool meet(const Piece& a, const Piece& b) { return a.n > 0 && b.n > 0 && a.p < b.p + b.n && b.p < a.p + a.n; }
+inline bool meet(const Piece& a, std::initializer_list<Piece> l) {
+  for (const Piece& b : l)
+    if (meet(a, b)) return true;
+  return false;
+}
 
 // lanes l ^ 1, l ^ 2 by quad permutes; after both, the halves of eight lanes by a mirror (the four lanes of a quad agree by then)
 template <int CTRL> __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {

@@ -110,6 +110,8 @@ int check_extent(const char* who, const void* t, int64_t ld, const void* codes, 
   const int64_t cpr = C / (16 / ts);
   S4F_CHECK(rows <= (int64_t)0xffffff * 256 * UNR / cpr, "%s: rows=%lld too large for one launch", who, (long long)rows);
   S4F_CHECK(ld == C || rows <= (int64_t)0xffffffffu / cpr, "%s: rows=%lld too large for a strided view", who, (long long)rows);
+  const Piece c = piece(codes, rows * C), s = piece(scales, rows * (C / ACTQ8_GROUP));
+  S4F_CHECK(!meet(piece(t, rows, ld, C, ts), {c, s}) && !meet(c, s), "%s: the activation, its codes and its scales overlap", who);
   return 0;
 }
 

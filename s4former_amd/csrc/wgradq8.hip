@@ -617,6 +617,18 @@ S4F_API int s4f_wgrad_packed(const s4f_wgrad_packed_desc* descs, int count, int 
   S4F_CHECK(need >= 0, "%s: sizes too large for one launch", who);
   S4F_CHECK(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need), "%s: workspace missing, misaligned or too small (%lld < %lld)",
             who, (long long)ws_bytes, (long long)need);
+  for (int i = 0; i < count; ++i) {
+    const Problem& p = a.p[i];
+    const Piece out = piece(p.out, (int64_t)p.M * p.N * 4), slabs = piece(ws, ws_bytes);
+    bool bad = meet(out, slabs);
+    for (int j = 0; j < count; ++j) {
+      const Problem& o = a.p[j];
+      const Piece dy = piece(o.dy, o.rows, o.lddy, o.M, dtype == S4F_BF16 ? 2 : 4), c = piece(o.codes, o.rows * o.N),
+                  s = piece(o.scales, o.rows * (o.N / ACTQ8_GROUP));
+      bad = bad || meet(out, {dy, c, s}) || meet(slabs, {dy, c, s}) || (j != i && meet(out, piece(o.out, (int64_t)o.M * o.N * 4)));
+    }
+    S4F_CHECK(!bad, "%s: an output or the workspace overlaps another or an input (problem %d)", who, i);
+  }
   bool join = false;
   int64_t n4 = 0;
   for (int i = 0; i < count; ++i)

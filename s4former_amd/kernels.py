@@ -734,12 +734,10 @@ def wgrad_packed(problems, dtype, ws=None, accumulate=True):
         elif not accumulate:
             out.zero_()
     wsp, wsb = _buf(ws, dev, 'wgrad_packed ws')
-    if wsb:
-        spans.append((wsp, wsp + wsb))
-    if len(spans) > 1:
+    if len(descs) < len(spans) > 1:                         # (problems without rows do not reach the entry point, which checks the others)
         spans.sort()
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise S4FError('wgrad_packed: outputs (or an output and the workspace) overlap')
+            raise S4FError('wgrad_packed: outputs overlap')
     if not descs:
         return
     arr = (L.WgradPackedDesc * len(descs))(*descs)

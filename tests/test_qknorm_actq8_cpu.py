@@ -139,6 +139,38 @@ def test_overlap_rule():
             ap(0, 192 if ldb == 192 else 64, pb, ldb, 4, 128, 2)
 
 
+FAR = 1 << 30          # apart from P by more than any of these tensors
+
+
+@pytest.mark.parametrize('change', [dict(codes=P + 512, scales=P + 2 * FAR), dict(codes=P + FAR, scales=P + 2046), dict(codes=P + FAR, scales=P + FAR + 1022),
+                                    dict(y=P + 3 * FAR, codes=P + 3 * FAR + 2032, scales=P + FAR)])
+def test_forward_entry_refuses_overlap(change):
+    # x and y: 8 rows of 256 bytes
+    refused('s4f_qk_norm_rope_fwd', {**FWD, **change}.values(), 'overlaps')
+
+
+@pytest.mark.parametrize('change', [dict(dgk=P + 5 * FAR + 252), dict(ws=P + FAR + 2032), dict(ws=P + 5 * FAR), dict(ws=P + 2 * FAR + 16), dict(dgq=P + FAR),
+                                    dict(x=None, codes=P + FAR + 16, scales=P + 8 * FAR), dict(x=None, codes=P + 8 * FAR, scales=P + FAR + 2046)])
+def test_backward_entry_refuses_overlap(change):
+    apart = dict(dy=P, x=P + 2 * FAR, dx=P + FAR, ws=P + 4 * FAR, dgq=P + 5 * FAR, dgk=P + 6 * FAR)
+    refused('s4f_qk_norm_rope_bwd', {**BWD, **apart, **change}.values(), 'overlap')
+
+
+@pytest.mark.parametrize('codes,scales', [(P + 512 - 16, P + FAR), (P - 256 + 16, P + FAR), (P + FAR, P + 511), (P + FAR, P + FAR + 255), (P, P + FAR)])
+def test_pack_entries_refuse_overlap(codes, scales):
+    # 4 rows of 64 bf16 values: 512 bytes, codes 256, scales 8
+    refused('s4f_act_pack', (P, 64, codes, scales, 4, 64, 1, None), 'overlap')
+    refused('s4f_act_unpack', (codes, scales, P, 64, 4, 64, 1, None), 'overlap')
+
+
+@pytest.mark.parametrize('second', [dict(out=P + 16), dict(dy=P + 4 * 64 * 64 - 16), dict(codes=P), dict(scales=P + 5), dict(dy=P + 9 * FAR + 16), dict(scales=P + 9 * FAR)])
+def test_wgrad_entry_refuses_overlap(second):
+    far = dict(dy=P + 2 * FAR, codes=P + 3 * FAR, scales=P + 4 * FAR, out=P + 5 * FAR, rows=16400)
+    first = dict(WG, dy=P + 6 * FAR, codes=P + 7 * FAR, scales=P + 8 * FAR, out=P, rows=16400)
+    arr = (L.WgradPackedDesc * 2)(L.WgradPackedDesc(**first), L.WgradPackedDesc(**{**WG, **far, **second}))
+    refused('s4f_wgrad_packed', (arr, 2, 1, 0, P + 9 * FAR, 1 << 28, None), 'overlap')
+
+
 # ------------------------------------------------------------------------------------------------------------- options of the backbone
 def test_backbone_options():
     import s4former_amd as S
