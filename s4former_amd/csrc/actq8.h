@@ -26,6 +26,13 @@ inline bool meet(const Piece& a, std::initializer_list<Piece> l) {
     if (meet(a, b)) return true;
   return false;
 }
+// two [rows, cols] matrices are the same one, or no element of one lies in the other (two column slices of one buffer, say)
+inline bool same_or_apart(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t rows, int64_t cols, int es) {
+  if ((a == b && (lda == ldb || rows == 1)) || !meet(piece(a, rows, lda, cols, es), piece(b, rows, ldb, cols, es))) return true;
+  if (lda != ldb || lda < 2 * cols) return false;
+  const int64_t ld = lda * es, d = (((const char*)b - (const char*)a) % ld + ld) % ld;
+  return d >= cols * es && d <= ld - cols * es;
+}
 
 // lanes l ^ 1, l ^ 2 by quad permutes; after both, the halves of eight lanes by a mirror (the four lanes of a quad agree by then)
 template <int CTRL> __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {

@@ -549,18 +549,6 @@ def _buf(t, dev, what):
     return t.data_ptr(), t.numel() * t.element_size()
 
 
-def _apart(pa, lda, pb, ldb, rows, row_bytes, es, what):
-    """the two [rows, row_bytes] matrices are the same one, or no element of one lies in the other"""
-    if pa == pb and lda == ldb:
-        return
-    lda, ldb = lda * es, ldb * es
-    if pa + (rows - 1) * lda + row_bytes <= pb or pb + (rows - 1) * ldb + row_bytes <= pa:
-        return
-    if lda == ldb and lda >= 2 * row_bytes and row_bytes <= (pb - pa) % lda <= lda - row_bytes:
-        return                                              # two column slices of one buffer
-    raise S4FError(f'{what} overlap')
-
-
 def _launch(name, *args):
     lib = L._lib
     if lib is None or L._prof is not None:
@@ -611,9 +599,6 @@ def qk_norm_rope_fwd(x, y, Hq, Hk, dtype, gq=None, gk=None, cos=None, sin=None, 
         yp, ldy, yrows = _mat(y, T, C, dev, 'qk_norm_rope_fwd y')
         if yrows != rows:
             raise S4FError(f'qk_norm_rope_fwd: x has {rows} rows, y {yrows}')
-        if xp != yp or ldx != ldy:
-            es = 2 if dtype == BF16 else 4
-            _apart(xp, ldx, yp, ldy, rows, C * es, es, 'qk_norm_rope_fwd: x and y')
     codes = scales = None
     if packed is not None:
         if gq is None:
@@ -638,30 +623,24 @@ def qk_norm_rope_bwd(dy, dx, Hq, Hk, dtype, x=None, packed=None, gq=None, gk=Non
     dxp, lddx, xrows = _mat(dx, T, C, dev, 'qk_norm_rope_bwd dx')
     if xrows != rows:
         raise S4FError(f'qk_norm_rope_bwd: dy has {rows} rows, dx {xrows}')
-    es = 2 if dtype == BF16 else 4
     xp = codes = scales = wsp = dgqp = dgkp = None
     ldx = wsb = 0
     if norm:
         if (x is None) == (packed is None) or dgq is None or dgk is None:
             raise S4FError('qk_norm_rope_bwd: the norm needs x or packed (not both), dgq and dgk')
         dgqp, dgkp = _vec(dgq, _F32T, 64, dev, 'qk_norm_rope_bwd dgq'), _vec(dgk, _F32T, 64, dev, 'qk_norm_rope_bwd dgk')
-        if abs(dgqp - dgkp) < 256:
-            raise S4FError('qk_norm_rope_bwd: dgq and dgk overlap')
         if packed is not None:
             codes, scales = _packed_ptrs(packed, rows, C, dev, 'qk_norm_rope_bwd')
         else:
             xp, ldx, xrows = _mat(x, T, C, dev, 'qk_norm_rope_bwd x')
             if xrows != rows:
                 raise S4FError(f'qk_norm_rope_bwd: dy has {rows} rows, x {xrows}')
-            if rows:
-                _apart(xp, ldx, dxp, lddx, rows, C * es, es, 'qk_norm_rope_bwd: x and dx')
         wsp, wsb = _buf(ws, dev, 'qk_norm_rope_bwd ws')
     if rows == 0:
         if norm and not accumulate:
             dgq.zero_(); dgk.zero_()
         return
     gq, gk, cos, sin, period = _gains_tables(rows, gq, gk, cos, sin, dev, 'qk_norm_rope_bwd')
-    _apart(dyp, lddy, dxp, lddx, rows, C * es, es, 'qk_norm_rope_bwd: dy and dx')
     _launch('s4f_qk_norm_rope_bwd', dyp, lddy, xp, ldx, codes, scales, dxp, lddx, gq, gk, cos, sin, period, eps, dgqp, dgkp,
             1 if accumulate else 0, wsp, wsb, rows, Hq, Hk, dtype, _stream_of(dev))
 

@@ -128,17 +128,6 @@ def test_front_refuses():
             call()
 
 
-def test_overlap_rule():
-    ap = lambda *a: K._apart(*a, 'x and y')                                                              # noqa: E731
-    ap(1000, 64, 1000, 64, 4, 128, 2)                       # the same matrix
-    ap(0, 64, 512, 64, 4, 128, 2)                           # one behind the other
-    ap(0, 192, 128, 192, 4, 128, 2)                         # neighbouring column slices of one buffer
-    ap(0, 192, 256, 192, 4, 128, 2)
-    for pb, ldb in ((2, 64), (128, 64), (64, 192), (0, 128), (384 - 64, 192)):
-        with pytest.raises(S4FError):
-            ap(0, 192 if ldb == 192 else 64, pb, ldb, 4, 128, 2)
-
-
 FAR = 1 << 30          # apart from P by more than any of these tensors
 
 
@@ -147,6 +136,22 @@ FAR = 1 << 30          # apart from P by more than any of these tensors
 def test_forward_entry_refuses_overlap(change):
     # x and y: 8 rows of 256 bytes
     refused('s4f_qk_norm_rope_fwd', {**FWD, **change}.values(), 'overlaps')
+
+
+# rows of 256 bytes: one element, half a row, a row on, other strides over the same memory, slices of one buffer that share columns
+MEET = [dict(y=P + 16), dict(y=P + 128), dict(y=P + 256), dict(y=P - 256), dict(ldx=384, ldy=384, y=P + 240), dict(ldx=384, ldy=384, y=P + 528),
+        dict(ldx=384, ldy=256), dict(ldx=0), dict(ldy=256), dict(ldx=192, ldy=192, y=P + 128)]
+
+
+@pytest.mark.parametrize('change', MEET)
+def test_rows_that_meet_are_refused(change):
+    refused('s4f_qk_norm_rope_fwd', {**FWD, **change}.values(), 'x and y overlap')
+    to = dict(x='dy', y='dx', ldx='lddy', ldy='lddx')
+    back = {to[k]: v for k, v in change.items()}
+    refused('s4f_qk_norm_rope_bwd', {**BWD, **dict(x=P + 2 * FAR, ws=P + 4 * FAR, dgq=P + 5 * FAR, dgk=P + 6 * FAR), **back}.values(), 'dy and dx overlap')
+    to = dict(x='x', y='dx', ldx='ldx', ldy='lddx')
+    back = {to[k]: v for k, v in change.items()}
+    refused('s4f_qk_norm_rope_bwd', {**BWD, **dict(dy=P + 2 * FAR, ws=P + 4 * FAR, dgq=P + 5 * FAR, dgk=P + 6 * FAR), **back}.values(), 'x and dx overlap')
 
 
 @pytest.mark.parametrize('change', [dict(dgk=P + 5 * FAR + 252), dict(ws=P + FAR + 2032), dict(ws=P + 5 * FAR), dict(ws=P + 2 * FAR + 16), dict(dgq=P + FAR),
@@ -169,6 +174,12 @@ def test_wgrad_entry_refuses_overlap(second):
     first = dict(WG, dy=P + 6 * FAR, codes=P + 7 * FAR, scales=P + 8 * FAR, out=P, rows=16400)
     arr = (L.WgradPackedDesc * 2)(L.WgradPackedDesc(**first), L.WgradPackedDesc(**{**WG, **far, **second}))
     refused('s4f_wgrad_packed', (arr, 2, 1, 0, P + 9 * FAR, 1 << 28, None), 'overlap')
+
+
+def test_rows_apart_pass_the_overlap_check():
+    # the same matrix, one behind the other, column slices of one buffer, a broadcast row in front of the output: the next check refuses
+    for change in (dict(), dict(y=P + 2048), dict(y=P - 2048), dict(ldx=384, ldy=384, y=P + 256), dict(ldx=384, ldy=384, y=P + 512), dict(ldx=0, y=P + 256)):
+        refused('s4f_qk_norm_rope_fwd', {**FWD, **change, 'codes': P + FAR, 'scales': P + FAR}.values(), 'checkpoint overlaps')
 
 
 # ------------------------------------------------------------------------------------------------------------- options of the backbone
