@@ -126,12 +126,11 @@ def _tables(case, gen):
 
 
 def _put_away(x):
-    """(codes int8, scales uint8) of a 32-bit tensor [rows, C]: code = round(x / s), s the least power of two that keeps |code| <= 127,
-    2^121 at most (there the codes stop at 127), so that what is restored stays finite"""
+    """(codes int8, scales uint8) of a 32-bit tensor [rows, C]: code = round(x / s), s the least power of two that keeps |code| <= 127"""
     g = x.reshape(x.shape[0], -1, GROUP)
     m, e = torch.frexp(g.abs().amax(-1))                     # amax = m 2^e, m in [0.5, 1)
-    e = torch.clamp(e - 7 + (m >= 255.0 / 256.0).to(e.dtype), -126, 121)
-    codes = torch.clamp(torch.round(torch.ldexp(g, -e[..., None])), -127, 127)
+    e = torch.clamp(e - 7 + (m >= 255.0 / 256.0).to(e.dtype), min=-126)
+    codes = torch.round(torch.ldexp(g, -e[..., None]))
     return codes.to(torch.int8).reshape(x.shape), (e + 127).to(torch.uint8)
 
 
@@ -291,14 +290,14 @@ def exact(case, seed):
         e = torch.floor(torch.log2(torch.clamp(big, min=2.0 ** -200)))
         e = e + (torch.exp2(e + 1) <= big).double() - (torch.exp2(e) > big).double()          # log2 next to a power of two
         e = e - 6
-        e = torch.clamp(torch.where(big / torch.exp2(e) >= 127.5, e + 1, e), -126, 121)
+        e = torch.clamp(torch.where(big / torch.exp2(e) >= 127.5, e + 1, e), min=-126)
         return torch.exp2(e).repeat_interleave(GROUP, 1)
 
     x = st['x'].double()
     kept = x
     if kind in ('ckpt', 'qk_step'):
         s = step(x)
-        kept = torch.clamp(torch.round(x / s), -127, 127) * s
+        kept = torch.round(x / s) * s
     if kind == 'ckpt':
         return kept
     rows, hq, hk = x.shape[0], case['Hq'], case['Hk']
