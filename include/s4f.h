@@ -205,7 +205,8 @@ int s4f_attention_bwd_fused(const void* qkv, const void* ctx, const void* dctx, 
  *   y_i = n_i c_i - n_{i+32} s_i, y_{i+32} = n_{i+32} c_i + n_i s_i   (i < 32; cos and sin given; NULL: no rotation, y = n)
  * cos / sin fp32 [period, 32], row r uses r % period (period = tokens per image: the images share positions; = rows: own ones).
  * eps: finite, a normal number.  Sums and products fp32, rounded once to T (a head whose squares leave fp32's range, |x| above about
- * 1e18, comes out as zeros).  y may be x itself (same ld).  All row starts 16-byte aligned.
+ * 1e18, comes out as zeros).  y may be x itself (same ld); apart from that nothing
+ * written (here and in the backward) may overlap anything else given to the call.  All row starts 16-byte aligned.
  * codes int8 [rows, (Hq + Hk) 64] and scales uint8 [rows, (Hq + Hk) 2] (both or NULL, norm only): an 8-bit checkpoint of the
  * pre-norm x in the format of s4f_act_pack. */
 int s4f_qk_norm_rope_fwd(const void* x, int64_t ldx, void* y, int64_t ldy, const float* gq, const float* gk, const float* cos,

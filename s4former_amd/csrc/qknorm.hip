@@ -265,6 +265,13 @@ int check_qk(const char* who, int64_t rows, int Hq, int Hk, int dtype, const flo
     S4F_CHECK((uintptr_t)p % 16 == 0, "%s: gains and tables must be 16-byte aligned", who);
   return 0;
 }
+// a piece of `written` has a byte in common with a gain or a table
+bool meet_params(const float* gq, const float* gk, const float* cos, const float* sin, int64_t period, std::initializer_list<Piece> written) {
+  const int64_t tab = cos ? period * 32 * 4 : 0;
+  for (const Piece& w : written)
+    if (meet(w, {piece(gq, 256), piece(gk, 256), piece(cos, tab), piece(sin, tab)})) return true;
+  return false;
+}
 int check_rows(const char* who, const char* what, const void* p, int64_t ld, int dtype) {
   S4F_CHECK(p, "%s: %s is null", who, what);
   S4F_CHECK((uintptr_t)p % 16 == 0 && ld >= 0 && ld % (dtype == S4F_BF16 ? 8 : 4) == 0, "%s: rows of %s must start on 16-byte boundaries", who, what);
@@ -309,6 +316,7 @@ S4F_API int s4f_qk_norm_rope_fwd(const void* x, int64_t ldx, void* y, int64_t ld
   const Piece px = piece(x, rows, ldx, C, es), py = piece(y, rows, ldy, C, es), pc = piece(codes, rows * C), ps = piece(scales, rows * C / 32);
   S4F_CHECK(same_or_apart(x, ldx, y, ldy, rows, C, es), "%s: x and y overlap", who);
   S4F_CHECK(!meet(pc, {px, py, ps}) && !meet(ps, {px, py}), "%s: the checkpoint overlaps x or y", who);
+  S4F_CHECK(!meet_params(gq, gk, cos, sin, period, {py, pc, ps}), "%s: y or the checkpoint overlaps the gains or the tables", who);
   QkArgs a{};
   a.x = x; a.ldx = ldx; a.y = y; a.ldy = ldy; a.gq = gq; a.gk = gk; a.cos = cos; a.sin = sin; a.codes = codes; a.scales = scales;
   a.eps = eps; a.rows = (uint32_t)rows; a.period = (uint32_t)(cos ? period : 1); a.Hq = Hq; a.H = Hq + Hk;
@@ -333,6 +341,8 @@ S4F_API int s4f_qk_norm_rope_bwd(const void* dy, int64_t lddy, const void* x, in
   S4F_CHECK(rows == 1 || lddx >= (int64_t)(Hq + Hk) * 64, "%s: rows of dx overlap", who);
   const int64_t C = (int64_t)(Hq + Hk) * 64;
   const int es = dtype == S4F_BF16 ? 2 : 4;
+  const Piece pd = piece(dx, rows, lddx, C, es), pw = piece(gq ? ws : nullptr, ws_bytes), pq = piece(gq ? dgq : nullptr, 256),
+              pk = piece(gq ? dgk : nullptr, 256);
   if (gq) {
     S4F_CHECK((codes != nullptr) == (scales != nullptr) && (codes != nullptr) != (x != nullptr), "%s: the norm's backward needs x or its checkpoint, not both", who);
     if (!codes)
@@ -341,13 +351,13 @@ S4F_API int s4f_qk_norm_rope_bwd(const void* dy, int64_t lddy, const void* x, in
     S4F_CHECK(dgq && dgk && ws && (uintptr_t)ws % 16 == 0, "%s: gain gradients and a 16-byte aligned workspace needed", who);
     S4F_CHECK(ws_bytes >= s4f_qk_ws_bytes(rows, Hq, Hk), "%s: workspace too small (%lld < %lld)", who, (long long)ws_bytes,
               (long long)s4f_qk_ws_bytes(rows, Hq, Hk));
-    const Piece pd = piece(dx, rows, lddx, C, es), pw = piece(ws, ws_bytes), pc = piece(codes, rows * C),
-                ps = piece(scales, rows * C / 32), pq = piece(dgq, 256), pk = piece(dgk, 256);
-    S4F_CHECK(!meet(pd, {pc, ps, pw, pq, pk}) && !meet(pw, {piece(dy, rows, lddy, C, es), piece(x, rows, ldx, C, es), pc, ps, pq, pk}) && !meet(pq, pk),
+    const Piece pc = piece(codes, rows * C), ps = piece(scales, rows * C / 32), py = piece(dy, rows, lddy, C, es), px = piece(x, rows, ldx, C, es);
+    S4F_CHECK(!meet(pd, {pc, ps, pw, pq, pk}) && !meet(pw, {py, px, pc, ps, pq, pk}) && !meet(pq, {pk, py, px, pc, ps}) && !meet(pk, {py, px, pc, ps}),
               "%s: dx, the gain gradients or the workspace overlap each other or an input", who);
     S4F_CHECK(codes || same_or_apart(x, ldx, dx, lddx, rows, C, es), "%s: x and dx overlap", who);
   }
   S4F_CHECK(same_or_apart(dy, lddy, dx, lddx, rows, C, es), "%s: dy and dx overlap", who);
+  S4F_CHECK(!meet_params(gq, gk, cos, sin, period, {pd, pw, pq, pk}), "%s: dx, the gain gradients or the workspace overlap the gains or the tables", who);
   QkArgs a{};
   a.dy = dy; a.lddy = lddy; a.x = x; a.ldx = ldx; a.y = dx; a.ldy = lddx; a.gq = gq; a.gk = gk; a.cos = cos; a.sin = sin;
   a.codes = gq ? const_cast<int8_t*>(codes) : nullptr; a.scales = const_cast<uint8_t*>(scales); a.part = (float*)ws; a.eps = eps;

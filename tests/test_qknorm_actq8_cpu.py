@@ -182,6 +182,37 @@ def test_rows_apart_pass_the_overlap_check():
         refused('s4f_qk_norm_rope_fwd', {**FWD, **change, 'codes': P + FAR, 'scales': P + FAR}.values(), 'checkpoint overlaps')
 
 
+# 8 rows of 256 bytes; gains of 256 bytes; tables of 4 positions, 512 bytes
+PAR = dict(gq=P + 9 * FAR, gk=P + 9 * FAR + 256, cos=P + 10 * FAR, sin=P + 10 * FAR + 512)
+ONTO = [('gq', 240), ('gk', 240), ('cos', 496), ('sin', 496), ('gq', 0), ('cos', 0)]
+
+
+@pytest.mark.parametrize('of,off', ONTO)
+def test_forward_refuses_writes_to_gains_and_tables(of, off):
+    at = PAR[of] + off
+    for change in (dict(y=at), dict(codes=at, scales=P + 3 * FAR), dict(codes=P + 3 * FAR, scales=at), dict(y=at - 2048 + 16)):
+        refused('s4f_qk_norm_rope_fwd', {**FWD, **PAR, 'y': P + 2 * FAR, **change}.values(), 'gains or the tables')
+    if of in ('cos', 'sin'):                                 # the rotation alone
+        refused('s4f_qk_norm_rope_fwd', {**FWD, **PAR, 'gq': None, 'gk': None, 'y': at}.values(), 'gains or the tables')
+
+
+@pytest.mark.parametrize('of,off', ONTO)
+def test_backward_refuses_writes_to_gains_and_tables(of, off):
+    at = PAR[of] + off
+    apart = {**BWD, **PAR, **dict(dy=P, x=P + 2 * FAR, dx=P + FAR, ws=P + 4 * FAR, dgq=P + 5 * FAR, dgk=P + 6 * FAR)}
+    for change in (dict(dx=at), dict(ws=at), dict(dgq=at), dict(dgk=at), dict(ws=at - (1 << 20) + 16)):
+        refused('s4f_qk_norm_rope_bwd', {**apart, **change}.values(), 'gains or the tables')
+    if of in ('cos', 'sin'):
+        refused('s4f_qk_norm_rope_bwd', {**apart, 'gq': None, 'gk': None, 'dx': at}.values(), 'gains or the tables')
+
+
+@pytest.mark.parametrize('change', [dict(dgq=P + 2032), dict(dgk=P + 2 * FAR), dict(x=None, codes=P + 7 * FAR, scales=P + 8 * FAR, dgq=P + 7 * FAR + 512),
+                                    dict(x=None, codes=P + 7 * FAR, scales=P + 8 * FAR, dgk=P + 8 * FAR + 16)])
+def test_backward_refuses_gain_gradients_over_inputs(change):
+    apart = {**BWD, **PAR, **dict(dy=P, x=P + 2 * FAR, dx=P + FAR, ws=P + 4 * FAR, dgq=P + 5 * FAR, dgk=P + 6 * FAR)}
+    refused('s4f_qk_norm_rope_bwd', {**apart, **change}.values(), 'overlap')
+
+
 # ------------------------------------------------------------------------------------------------------------- options of the backbone
 def test_backbone_options():
     import s4former_amd as S
