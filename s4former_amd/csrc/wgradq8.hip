@@ -15,6 +15,14 @@ namespace {
 
 constexpr int MAXP = 4;
 
+// Offsets into the rows of a step are unsigned.  A column outside the matrix gets OUTSIDE, which stays beyond every resource (at most 2^30
+// bytes: 64 rows of 2^24 or 128 of 2^23) whatever is added for a later row of the step (less than 2^30) or taken for the other half of a chunk
+constexpr uint32_t OUTSIDE = 0x80000000u, MOST = 1u << 30;
+// 16 codes come as two halves of eight; where `hb`, the upper one first: offset of the second
+constexpr uint32_t second_half(uint32_t first, int hb) { return hb ? first - 8 : first + 8; }
+static_assert(second_half(OUTSIDE, 0) >= MOST && second_half(OUTSIDE, 1) >= MOST && second_half(OUTSIDE, 0) + MOST > OUTSIDE,
+              "a column outside reads as zero from both halves, in every row of a step");
+
 struct Problem {
   const void* dy; int64_t lddy;
   const int8_t* codes; const uint8_t* scales;
@@ -72,11 +80,10 @@ __global__ __launch_bounds__(256, 2) void wgrad_f32_kernel(const Args args) {
   // a thread's block: rows 4 rg .. + 3, columns c4 .. + 3 of dY and of the codes (M is a multiple of 8 and N of 32: inside or outside).  The
   // resources cover the rows of the step, so rows behind the range read as zero; columns outside get an offset beyond every resource
   const int rg = tid >> 4, c4 = (tid & 15) * 4;
-  const int OUT = (int)0x80000000;
   const int ld4 = (int)(P.lddy * 4);
-  const int va = m0 + c4 < M ? 4 * rg * ld4 + (m0 + c4) * 4 : OUT;
-  const int vb = n0 + c4 < N ? 4 * rg * N + n0 + c4 : OUT;
-  const int vs = n0 + c4 < N ? 4 * rg * ns + (n0 + c4) / ACTQ8_GROUP : OUT;
+  const uint32_t va = m0 + c4 < M ? 4 * rg * ld4 + (m0 + c4) * 4 : OUTSIDE;
+  const uint32_t vb = n0 + c4 < N ? 4 * rg * N + n0 + c4 : OUTSIDE;
+  const uint32_t vs = n0 + c4 < N ? 4 * rg * ns + (n0 + c4) / ACTQ8_GROUP : OUTSIDE;
   const int64_t r_beg = (int64_t)k_beg * BKR;
   int left = (int)(min(P.rows, (int64_t)k_end * BKR) - r_beg);
   char* pa = (char*)P.dy + r_beg * ld4;
@@ -233,11 +240,10 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void wgrad_bf16_kernel(const 
   // the range read as zero; columns outside are given an offset beyond every resource.  16 codes come as two loads of 8: four of each
   // eight lanes take (and store) the upper half first, so that the eight 16-byte stores served at once touch different banks
   const int ra = tid / CA, ua = (tid % CA >> 2) ^ place<TM>(ra), ca = 4 * ua + (tid & 3), rb = tid / CB, cb = tid % CB, hb = (tid >> 2) & 1;
-  const int OUT = (int)0x80000000;
   const int ld2 = (int)(P.lddy * 2), ns = N / ACTQ8_GROUP;
-  const int va = m0 + 8 * ca < M ? ra * ld2 + (m0 + 8 * ca) * 2 : OUT;
-  const int vb = n0 + 16 * cb < N ? rb * N + n0 + 16 * cb + 8 * hb : OUT, vb2 = vb + 8 - 16 * hb;
-  const int vs = n0 + 16 * cb < N ? rb * ns + (n0 + 16 * cb) / ACTQ8_GROUP : OUT;
+  const uint32_t va = m0 + 8 * ca < M ? ra * ld2 + (m0 + 8 * ca) * 2 : OUTSIDE;
+  const uint32_t vb = n0 + 16 * cb < N ? rb * N + n0 + 16 * cb + 8 * hb : OUTSIDE, vb2 = second_half(vb, hb);
+  const uint32_t vs = n0 + 16 * cb < N ? rb * ns + (n0 + 16 * cb) / ACTQ8_GROUP : OUTSIDE;
   struct Regs { u32x2 b[NB][2]; uint32_t s[NB]; } R[2];
   const int64_t r_beg = (int64_t)k_beg * STEP;
   int left = (int)(min(P.rows, (int64_t)k_end * STEP) - r_beg);
