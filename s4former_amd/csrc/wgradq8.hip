@@ -587,7 +587,7 @@ template <int MI, int NI, int WM, int WN, int KG = 1> void launch_bf16(const Arg
 
 // dims: {dtype, then M, N, rows of each problem}
 int64_t s4f_wgrad_packed_ws(const int64_t* dims, int ndims) {
-  if (ndims < 4 || (ndims - 1) % 3 || (ndims - 1) / 3 > MAXP) return -1;
+  if (ndims < 4 || (dims[0] != S4F_F32 && dims[0] != S4F_BF16) || (ndims - 1) % 3 || (ndims - 1) / 3 > MAXP) return -1;
   Args a{};
   a.count = (ndims - 1) / 3;
   for (int i = 0; i < a.count; ++i) {

@@ -213,6 +213,12 @@ def test_backward_refuses_gain_gradients_over_inputs(change):
     refused('s4f_qk_norm_rope_bwd', {**apart, **change}.values(), 'overlap')
 
 
+@pytest.mark.parametrize('dtype', [-1, 2, 1 << 32])
+def test_workspace_query_refuses_types(dtype):
+    with pytest.raises(S4FError):
+        K.workspace_bytes(K.WS_WGRAD_PACKED, dtype, 64, 64, 4096)
+
+
 # ------------------------------------------------------------------------------------------------------------- options of the backbone
 def test_backbone_options():
     import s4former_amd as S
