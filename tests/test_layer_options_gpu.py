@@ -210,6 +210,33 @@ def test_backward_from_checkpoints(dtype, residual, qk_norm, theta):
         close(got[n].grad, r, TOL[dtype], n)
 
 
+@pytest.mark.parametrize('dtype,residual', [('fp32', 'fp32'), ('bf16', 'fp32'), ('bf16', 'bf16')], indirect=['residual'])
+@pytest.mark.parametrize('theta', [100.0, None])
+def test_norm_backward_without_checkpoints(dtype, residual, theta):
+    """one layer with qk_norm alone: queries and keys in front of the norm are kept in their own type and tensor; the gradients are the
+    formulas' on what was kept"""
+    m = make_vit(dtype, layers=1, img=64, qk_norm=True, rope_theta=theta)
+    x = torch.randn(3, 3, 64, 64, generator=torch.Generator().manual_seed(5)).cuda()
+    out = m(x)[0]
+    (node,) = saved_layers(out)
+    sv = dict(node.sv)
+    B, N, E = 3, 17, 256
+    assert torch.is_tensor(sv['pre']) and sv['pre'].shape == (B * N, 2 * E) and torch.is_tensor(sv['a'])
+    go = torch.randn(out.shape, generator=torch.Generator().manual_seed(8)).to(out.dtype).cuda()
+    g2 = torch.zeros(B, N, E, dtype=torch.float64)
+    g2[:, 1:] = go.detach().cpu().double().flatten(2).transpose(1, 2)
+    prm = dict(m.layers[0].named_parameters())
+    if dtype == 'bf16':
+        prm = {n: (p.detach().bfloat16().float() if p.dim() == 2 else p) for n, p in prm.items()}
+    ref, _ = layer_backward(sv, prm, g2, B, N, E, 4, True, m._rope((4, 4), x.device))
+    out.backward(go)
+    torch.cuda.synchronize()
+    got = dict(m.layers[0].named_parameters())
+    assert set(ref) == set(got)
+    for n, r in ref.items():
+        close(got[n].grad, r, TOL[dtype], n)
+
+
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
 def test_forward_is_untouched_and_less_is_kept(dtype):
     x = torch.randn(2, 3, 96, 96, generator=torch.Generator().manual_seed(5)).cuda()
@@ -262,6 +289,45 @@ def test_options_in_the_training_step(dtype):
     for n in names:
         if n.startswith('backbone.'):
             assert not torch.equal(now[n], start[n]), n
+
+
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
+def test_teacher_gains_are_the_moving_average(dtype):
+    """every step in front of the teacher's pass: gain <- m gain + (1 - m) the student's gain, for each of the teacher's gains.  m and 1 - m,
+    the product and the sum are rounded once each: 4 half steps of the magnitudes"""
+    S.set_compute_dtype(dtype)
+    cfg = C.tiny_model_cfg(unsup_weight=1.0, attn_mask_seperate_head=True, attn_mask_weight=5, adaptive_attn_mask=True)
+    for k in ('backbone', 'backbone_ema'):
+        cfg[k].update(qk_norm=True, rope_theta=100.0, act_q8=True)
+    model = S.build_segmentor(cfg)
+    model.train()
+    C.load_filled(model, 1999, 60.0)
+    model.cuda()
+    opt = S.build_optimizer(model, dict(OPT))
+    gains = [n for n, _ in model.named_parameters() if n.startswith('backbone.') and n.endswith(('q_norm.weight', 'k_norm.weight'))]
+    assert len(gains) == 2 * 4
+    m = model.momentum_backbone
+    assert 0 < m < 1
+
+    def values(prefix):
+        now = dict(model.named_parameters())
+        return {n: now[n.replace('backbone.', prefix, 1)].detach().double().cpu().clone() for n in gains}
+    for it in range(3):
+        imgs, gt, metas = C.make_batch(2024 + it, 2, 2)
+        student, teacher = values('backbone.'), values('backbone_ema.')
+        opt.zero_grad()
+        C.seed_host_rng(2024 + it)
+        out = model.train_step(dict(img=imgs.cuda(), img_metas=metas, gt_semantic_seg=gt.cuda()), opt, iter=it)
+        torch.cuda.synchronize()
+        after = values('backbone_ema.')
+        for n in gains:
+            want, mag = m * teacher[n] + (1 - m) * student[n], m * teacher[n].abs() + (1 - m) * student[n].abs()
+            assert bool(((after[n] - want).abs() <= 4 * 2.0 ** -24 * mag).all()), (it, n)
+            moved = (1 - m) * (student[n] - teacher[n])
+            assert float(moved.abs().max()) > 16 * 2.0 ** -24 * float(mag.max()), 'the values are too close for a skipped update to show'
+        out['loss'].backward()
+        opt.step()
+        torch.cuda.synchronize()
 
 
 def test_second_backward_is_refused():

@@ -251,6 +251,85 @@ def test_qk_backward_against_differences(K, norm, rope):
         assert abs(num - ana) <= 1e-5 * (dg[0].cpu().double() * d).abs().sum(), (num, ana)
 
 
+# B, N, Hq, Hk: so many heads that the backward's grid is capped, a lane takes several of them (a ragged number) and the join of the gains
+# more than one turn
+MANY_CASES = [(8, 1025, 12, 12), (3, 2305, 16, 4)]
+
+
+def kind_blocks(rows, heads, all_heads, packed, code):
+    """(blocks of the backward for the heads of one kind, heads that a block takes at a time)"""
+    per, most = 64 if packed and code == 1 else 32, 1024 if packed else 768
+    return min(-(-rows * heads // per), max(1, most * heads // all_heads)), per
+
+
+def many_gain_steps(rows, heads, all_heads, packed, code):
+    blocks, per = kind_blocks(rows, heads, all_heads, packed, code)
+    lane, turns = -(-rows * heads // (blocks * per)), -(-blocks // 256)
+    # u and dz (60); a lane's own heads; the lanes of a wave (at most 4 exchanges) and its 4 waves; the join: a thread's turns, 6 exchanges, 4 waves
+    return 60 + lane + 4 + 4 + turns + 6 + 4
+
+
+@pytest.mark.parametrize('code', DTYPES)
+@pytest.mark.parametrize('packed', [False, True])
+@pytest.mark.parametrize('case', MANY_CASES)
+def test_many_heads_backward(K, code, packed, case):
+    """dx and the gains' gradients at sizes of a real batch, each kind of head by its own number of blocks"""
+    B, N, Hq, Hk = case
+    rows, H, C, eps = B * N, Hq + Hk, (Hq + Hk) * 64, 1e-6
+    blocks = [kind_blocks(rows, h, H, packed, code) for h in (Hq, Hk)]
+    assert max(b for b, _ in blocks) > 256 and all(rows * h > b * per for (b, per), h in zip(blocks, (Hq, Hk)))
+    gen = torch.Generator(device='cuda').manual_seed(rows)
+    x = (torch.randn(rows, C, device='cuda', generator=gen) * torch.exp(0.3 * torch.randn(1, C, device='cuda', generator=gen))).to(tdt(code))
+    dy = (0.1 * torch.randn(rows, C, device='cuda', generator=gen)).to(tdt(code))
+    gq, gk = [1 + 0.3 * torch.randn(64, device='cuda', generator=gen) for _ in range(2)]
+    cos, sin = [t.cuda() for t in tables(N)]
+    kept, kw = x.double(), dict(x=x)
+    if packed:
+        codes, scales = torch.empty(rows, C, device='cuda', dtype=torch.int8), torch.empty(rows, C // 32, device='cuda', dtype=torch.uint8)
+        K.act_pack(x, codes, scales, code)
+        kept, kw = q8_restore(codes.double(), torch.exp2(scales.double() - 127)), dict(packed=(codes, scales))
+    dx = torch.empty_like(x)
+    dg = [torch.full((64,), float('nan'), device='cuda') for _ in range(2)]
+    ws = torch.full((K.qk_norm_rope_ws_bytes(rows, Hq, Hk) // 4,), float('nan'), device='cuda')
+    par = dict(gq=gq, gk=gk, cos=cos, sin=sin, eps=eps, ws=ws)
+    K.qk_norm_rope_bwd(dy, dx, Hq, Hk, code, dgq=dg[0], dgk=dg[1], accumulate=False, **kw, **par)
+    rdx, mdx, rq, mq, rk, mk = qk_plain_bwd(dy, kept, Hq, Hk, gq, gk, cos, sin, eps)
+    within(dx, rdx.cpu(), (half(code) * rdx.abs() + BWD_STEPS * U * mdx * (1 + half(code))).cpu(), 'dx')
+    steps = [many_gain_steps(rows, h, H, packed, code) for h in (Hq, Hk)]
+    within(dg[0], rq.cpu(), (steps[0] * U * mq).cpu(), 'dgq')
+    within(dg[1], rk.cpu(), (steps[1] * U * mk).cpu(), 'dgk')
+    before = [g.clone() for g in dg]
+    K.qk_norm_rope_bwd(dy, dx, Hq, Hk, code, dgq=dg[0], dgk=dg[1], **kw, **par)                       # added: one more rounding
+    for g, b in zip(dg, before):
+        assert torch.equal(g, b + b)
+
+
+@pytest.mark.parametrize('code', DTYPES)
+@pytest.mark.parametrize('packed', [False, True])
+@pytest.mark.parametrize('case', MANY_CASES)
+def test_gain_sums_lose_nothing(K, code, packed, case):
+    """x of +1 and -1 (mean 1, an eps that vanishes beside it: u = x), whole dy and quarter turns: every operation is exact and every sum a whole
+    number below 2^24, so one head that is left out or taken twice shows"""
+    B, N, Hq, Hk = case
+    rows, H, C = B * N, Hq + Hk, (Hq + Hk) * 64
+    gen = torch.Generator(device='cuda').manual_seed(rows + 1)
+    x = (torch.randint(0, 2, (rows, C), device='cuda', generator=gen) * 2 - 1).to(tdt(code))
+    dy = torch.randint(-3, 4, (rows, C), device='cuda', generator=gen).to(tdt(code))
+    quarter = torch.randint(0, 4, (N, 32), device='cuda', generator=gen)
+    cos, sin = [torch.tensor(v, device='cuda')[quarter] for v in ([1.0, 0.0, -1.0, 0.0], [0.0, 1.0, 0.0, -1.0])]
+    gain = torch.ones(64, device='cuda')
+    kw = dict(x=x)
+    if packed:
+        kw = dict(packed=(torch.empty(rows, C, device='cuda', dtype=torch.int8), torch.empty(rows, C // 32, device='cuda', dtype=torch.uint8)))
+        K.act_pack(x, *kw['packed'], code)
+    dx = torch.empty_like(x)
+    dg = [torch.empty(64, device='cuda') for _ in range(2)]
+    ws = torch.empty(K.qk_norm_rope_ws_bytes(rows, Hq, Hk), device='cuda', dtype=torch.uint8)
+    K.qk_norm_rope_bwd(dy, dx, Hq, Hk, code, gq=gain, gk=gain, cos=cos, sin=sin, eps=2.0 ** -126, dgq=dg[0], dgk=dg[1], ws=ws, accumulate=False, **kw)
+    each = (turn(dy.double().reshape(rows, H, 64), cos, sin, -1.0) * x.double().reshape(rows, H, 64)).sum(0)
+    assert torch.equal(dg[0].double(), each[:Hq].sum(0)) and torch.equal(dg[1].double(), each[Hq:].sum(0))
+
+
 # ------------------------------------------------------------------------------------------------------------- checkpoints
 PACK_CASES = [(1, 32, 0), (1, 352, 8), (3, 64, 0), (65, 768, 0), (7, 1056, 8), (130, 256, 640), (1025, 96, 32)]
 
