@@ -469,11 +469,12 @@ def _plan_backward_ready(plan, store, prm, code, dev):
 class LayerOpt:
     """What an encoder layer does beyond the reference's: norm - RMS norm of queries and keys per head (two gain parameters behind the
     layer's twelve); cos, sin - rotation of queries and keys by the position of their token ([tokens, 32] tables); q8 - the activations
-    that only the backward pass reads are kept in 8 bits (kernels.act_pack) instead of their own type."""
-    __slots__ = ('norm', 'cos', 'sin', 'q8')
+    that only the backward pass reads are kept in 8 bits (kernels.act_pack) instead of their own type; grad - a backward pass may follow (the
+    caller's grad mode: needs_input_grad tells only which inputs ask for gradients)."""
+    __slots__ = ('norm', 'cos', 'sin', 'q8', 'grad')
 
-    def __init__(self, norm=False, cos=None, sin=None, q8=False):
-        self.norm, self.cos, self.sin, self.q8 = norm, cos, sin, q8
+    def __init__(self, norm=False, cos=None, sin=None, q8=False, grad=True):
+        self.norm, self.cos, self.sin, self.q8, self.grad = norm, cos, sin, q8, grad
 
     @property
     def qk(self):
@@ -550,7 +551,9 @@ class LayerFn(Function):
         dev = x.device
         x = x.contiguous()
         R = x.dtype
-        need_grad = any(ctx.needs_input_grad)
+        need_grad = any(ctx.needs_input_grad) and (opt is None or opt.grad)
+        if opt is not None and not (opt.qk or need_grad):
+            opt = None                                       # checkpoints alone, and nothing to keep: the plain layer
         xn = torch.empty(M, E, device=dev, dtype=T)
         mean1 = torch.empty(M, device=dev); rstd1 = torch.empty(M, device=dev)
         qkv = torch.empty(M, 3 * E, device=dev, dtype=T)

@@ -144,9 +144,10 @@ class TransformerEncoderLayer(BaseModule):
         if attn_mask is not None:
             bu, rf, bw = attn_mask
         opt = None
-        if self.qk_norm or self.act_q8 or rope is not None:
+        grad = torch.is_grad_enabled()                       # (inside LayerFn it never is)
+        if self.qk_norm or rope is not None or (self.act_q8 and grad):
             cos, sin = rope if rope is not None else (None, None)
-            opt = LayerOpt(self.qk_norm, cos, sin, self.act_q8)
+            opt = LayerOpt(self.qk_norm, cos, sin, self.act_q8, grad)
         return LayerFn.apply(x, bu, rf, float(bw), self.num_heads, self.eps, store, opt, *self._params())
 
 

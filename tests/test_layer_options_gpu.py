@@ -330,6 +330,40 @@ def test_teacher_gains_are_the_moving_average(dtype):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize('how', ['no_grad', 'inference_mode', 'frozen'])
+@pytest.mark.parametrize('qk_norm', [False, True])
+def test_nothing_is_kept_without_a_backward(monkeypatch, qk_norm, how):
+    """a pass that no backward follows (teacher, inference, frozen parameters): nothing is packed or put aside; with act_q8 alone the layer is
+    the plain one, with its one call a layer"""
+    from s4former_amd import functional as Fn
+    m = make_vit('fp32', qk_norm=qk_norm, act_q8=True)
+    x = torch.randn(2, 3, 64, 64, generator=torch.Generator().manual_seed(5)).cuda()
+    ref = [o.detach().clone() for o in m(x)]
+    names, in_place = [], []
+    call, norm = Fn.L.call, Fn.K.qk_norm_rope_fwd
+
+    def spy_norm(a, b, *args, packed=None, **kw):
+        in_place.append(a is b and packed is None)
+        return norm(a, b, *args, packed=packed, **kw)
+    monkeypatch.setattr(Fn.L, 'call', lambda name, *a, **k: (names.append(name), call(name, *a, **k))[1])
+    monkeypatch.setattr(Fn.K, 'act_pack', lambda *a: names.append('act_pack'))
+    monkeypatch.setattr(Fn.K, 'qk_norm_rope_fwd', spy_norm)
+    if how == 'frozen':
+        for p in m.parameters():
+            p.requires_grad_(False)
+        out = m(x)
+    else:
+        with getattr(torch, how)():
+            out = m(x)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, ref))
+    assert 'act_pack' not in names
+    if qk_norm:
+        assert in_place == [True, True]
+    else:
+        assert names.count('s4f_encoder_layer_fwd') == 2
+
+
 def test_second_backward_is_refused():
     m = make_vit('fp32', layers=1, act_q8=True)
     out = m(torch.zeros(1, 3, 64, 64, device='cuda'))[0]
