@@ -151,6 +151,10 @@ class TransformerEncoderLayer(BaseModule):
         return LayerFn.apply(x, bu, rf, float(bw), self.num_heads, self.eps, store, opt, *self._params())
 
 
+# patch grids whose rotation tables a backbone keeps (256 bytes a token); the tables of further ones are made for each call
+ROPE_GRIDS = 64
+
+
 def axial_rope_tables(h, w, theta, device):
     """cos and sin fp32 [1 + h w, 32] of the rotation of queries and keys on an h x w patch grid: pairs 0..15 of a head turn with the patch's
     row, pairs 16..31 with its column, by theta^(-i / 16) radians a patch; the cls token is not turned.  Angles in 64 bits."""
@@ -339,9 +343,12 @@ class VisionTransformer(BaseModule):
         if self.rope_theta is None:
             return None
         key = (*hw, torch.device(device))
-        if key not in self._rope_tables:
-            self._rope_tables[key] = axial_rope_tables(*hw, self.rope_theta, device)
-        return self._rope_tables[key]
+        tab = self._rope_tables.get(key)
+        if tab is None:
+            tab = axial_rope_tables(*hw, self.rope_theta, device)
+            if len(self._rope_tables) < ROPE_GRIDS:          # (a kept table is never dropped: another stream or a graph may read it)
+                self._rope_tables[key] = tab
+        return tab
 
     def forward_rank1(self, inputs, mask=None, tap_groups=None):
         """forward with the PASA mask already in rank-1 form (bias_u [B,N], row_flag [B,N] | None, weight) | None.

@@ -256,3 +256,14 @@ def test_axial_tables():
     t = 1 + row * 5 + col
     a, b = torch.tensor(row * 100.0 ** (-i / 16), dtype=torch.float64), torch.tensor(col * 100.0 ** (-i / 16), dtype=torch.float64)
     assert cos[t, i] == a.cos().float() and sin[t, i] == a.sin().float() and cos[t, 16 + i] == b.cos().float() and sin[t, 16 + i] == b.sin().float()
+
+
+def test_rotation_tables_do_not_pile_up():
+    from s4former_amd import vit
+    m = vit.VisionTransformer(img_size=64, embed_dims=128, num_layers=1, num_heads=2, rope_theta=100.0)
+    grids = [(h, w) for h in range(1, 13) for w in range(1, 13)]
+    for hw in grids * 2:
+        got, want = m._rope(hw, 'cpu'), vit.axial_rope_tables(*hw, 100.0, 'cpu')
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert len(m._rope_tables) == vit.ROPE_GRIDS < len(grids)
+    assert m._rope(grids[0], 'cpu')[0] is m._rope(grids[0], 'cpu')[0]              # a kept one is the same each time
