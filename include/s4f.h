@@ -223,7 +223,8 @@ int s4f_qk_norm_rope_bwd(const void* dy, int64_t lddy, const void* x, int64_t ld
 /* ------------------------------------------------------------------------------------------- activation checkpoints in 8 bits
  * x T [rows, C] (row stride ldx) -> codes int8 [rows, C], scales uint8 [rows, C / 32]: groups of 32 channels share the least power
  * of two s with round(max |x| / s) <= 127 (2^-126 .. 2^121), code = round-to-even(x / s), scale byte = exponent of s + 127; 255
- * marks a group that holds an infinity or a NaN (restored as NaN).  |x - code s| <= max |x| / 127.5; code s is exact in bf16. */
+ * marks a group that holds an infinity or a NaN (restored as NaN).  |x - code s| <= the larger of max |x| / 127.5 and 2^-127 (half the
+ * least s: a group below 2^-127 comes back as zeros); code s is exact in bf16. */
 int s4f_act_pack(const void* x, int64_t ldx, int8_t* codes, uint8_t* scales, int64_t rows, int C, int dtype, s4f_stream stream);
 /* y T [rows, C] (row stride ldy) = code s */
 int s4f_act_unpack(const int8_t* codes, const uint8_t* scales, void* y, int64_t ldy, int64_t rows, int C, int dtype, s4f_stream stream);

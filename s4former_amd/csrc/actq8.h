@@ -2,10 +2,10 @@
 //
 //   amax = max |x| over the group,  s = the least power of two with round(amax / s) <= 127,  code = round-to-even(x / s)
 //
-// x / s and code * s are exact (a shift of the exponent), so |x - code s| <= s / 2 with amax / 127.5 < s <= amax / 63.75, and
-// code * s has at most seven significant bits: it is exact in bf16, a restored value or matrix operand is never rounded again.
-// s stops at 2^-126 below and at 2^121 above, where codes stop at 127 (with 2^122 the largest magnitudes would restore as infinity);
-// |x - code s| <= amax / 127.5 holds there too.
+// x / s and code * s are exact (a shift of the exponent), so |x - code s| <= s / 2, and code * s has at most seven significant bits: it is
+// exact in bf16, a restored value or matrix operand is never rounded again.  Where s is not clamped, amax / 127.5 < s <= amax / 63.75 and
+// the error is at most amax / 127.5.  s stops at 2^121 above, where codes stop at 127 (with 2^122 the largest magnitudes would restore as
+// infinity) and the bound stands, and at 2^-126 below, where it is 2^-127 instead: a group of magnitudes up to 2^-127 restores as zeros.
 // The scale byte is the biased exponent of s (1 .. 248; groups of zeros take 1); 255 marks a group that
 // held an infinity or a NaN: all its 32 values come back as NaN, so that a diverged pass is not hidden.  Byte 0 is never written and
 // stands for zeros.

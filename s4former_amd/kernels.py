@@ -671,7 +671,8 @@ def _ckpt(t, codes, scales, dtype, what):
 
 def act_pack(x, codes, scales, dtype):
     """8-bit checkpoint of x [rows, C] (C a multiple of 32; a column slice of a wider buffer qualifies): codes int8 [rows, C], scales uint8
-    [rows, C / 32].  |x - restored| <= max |x| / 127.5 over the 32 channels; a group with an infinity or a NaN comes back as NaN."""
+    [rows, C / 32].  |x - restored| <= max(max |x| / 127.5, 2^-127), max |x| over the 32 channels; a group with an infinity or a NaN comes
+    back as NaN."""
     xp, ldx, cp, sp, rows, C, dev = _ckpt(x, codes, scales, dtype, 'act_pack')
     if rows:
         _launch('s4f_act_pack', xp, ldx, cp, sp, rows, C, dtype, _stream_of(dev))
