@@ -247,7 +247,7 @@ __global__ __launch_bounds__(64 * NW, (QT == 4) ? 2 : ((NW == 8 && sizeof(T) == 
         const f32x4 uu = *reinterpret_cast<const f32x4*>(us + ks * 16 + 4 * g);
         const f32x4 k4 = f32x4{kScale2, kScale2, kScale2, kScale2};
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) st[ks][qt] = __builtin_elementwise_fma(st[ks][qt], k4, uu * flagq[qt]);   // packed fp32
+        for (int qt = 0; qt < QT; ++qt) st[ks][qt] = __builtin_elementwise_fma(st[ks][qt], k4, uu * flagq[qt]);   // four scores at a time
       }
     }
     if (ragged) {
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(64 * NW, (QT == 4) ? 2 : ((NW == 8 && sizeof(T) == 
       f32x4 ps4 = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        const f32x4 e = HAS_BIAS ? st[ks][qt] + mc4 : __builtin_elementwise_fma(st[ks][qt], kc4, mc4);   // packed fp32
+        const f32x4 e = HAS_BIAS ? st[ks][qt] + mc4 : __builtin_elementwise_fma(st[ks][qt], kc4, mc4);   // four scores at a time
 #pragma unroll
         for (int r = 0; r < 4; ++r) st[ks][qt][r] = fexp2<T>(e[r]);
         ps4 += st[ks][qt];
