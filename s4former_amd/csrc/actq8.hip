@@ -2,8 +2,8 @@
 //
 // Both are one pass bound by HBM: 16 bytes of T per lane and access (8 bf16 / 4 fp32), a group of 32 spread over 4 / 8 lanes, so
 // that a wave reads and writes whole lines and the group's maximum takes two or three lane exchanges without LDS.
-// Measured, bf16, 8,200 x 4,096: pack 16.3 us, unpack 15.4 us with the tensors in the last-level cache (6.2 and 6.6 TB/s), both
-// together 40.7 us on fresh ones (5.0 TB/s, the rate of a large copy).
+// Measured at 8,200 x 4,096, calls one behind the other on the same tensors (in the last-level cache) / on fresh ones: bf16 pack 16.1 /
+// 20.2 us, unpack 15.3 / 21.5 us (6.3 and 6.7 / 5.0 and 4.7 TB/s; a large copy 4.8 - 5.0), fp32 pack 24.4 / 31.0 us, unpack 25.5 / 33.3 us.
 #include "actq8.h"
 #include "../../include/s4f.h"
 

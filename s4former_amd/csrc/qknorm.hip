@@ -10,13 +10,15 @@
 // Layout: LANES lanes hold a head; a lane has V = 32 / LANES values of the lower and V of the upper half, so that a rotation's pair stays in
 // the lane, the mean takes two or three lane exchanges, and one 8-bit group (32 channels: a half) is spread over the same lanes.  Four
 // lanes and 16-byte accesses for bf16, eight for fp32; eight also for the backward from x, whose registers then leave room for twice the
-// waves (3 x 2,305 rows, 16 + 4 heads: 14.3 us, with four lanes 15.6; from the checkpoint four are faster by 2 us at 16,400 rows x 24).
-// Both passes are bound by HBM; the tables (256 bytes a row) are read per head but come from cache, the heads of a row being
+// waves (3 x 2,305 rows, 16 + 4 heads, with the join: 13.7 us, with four lanes 15.3; from the checkpoint four are faster by 2 us at 16,400
+// rows x 24).  Both passes are bound by HBM; the tables (256 bytes a row) are read per head but come from cache, the heads of a row being
 // neighbours in the grid.
 //
-// Measured, bf16, 16,400 rows x 24 heads: forward 17.4 us with the tensors in the last-level cache (6.0 TB/s) and 23.3 us on fresh ones
-// (4.5 TB/s; a large copy reaches 4.8 - 5.0), with the checkpoint 21.9 us; backward 25.7 us from the checkpoint and 27.8 us from x,
-// 4 us of them the join of the gains.  A call on few rows takes 2.5 - 3.5 us on the GPU, less than its launch costs the host.
+// Measured at 16,400 rows x 24 heads, calls one behind the other on the same tensors (partly in the last-level cache) / on fresh ones, the
+// backward with the join of the gains (4 us; a large copy reaches 4.8 - 5.0 TB/s):
+//   bf16  forward 16.6 / 21.9 us (6.1 / 4.6 TB/s), with the checkpoint 21.7 / 28.9, backward from x 27.7 / 33.5, from the checkpoint 25.4 / 32.1
+//   fp32  forward 29.6 / 36.6 us (6.8 / 5.5 TB/s), with the checkpoint 34.1 / 41.3, backward from x 51.2 / 59.2, from the checkpoint 39.4 / 46.5
+// A call on few rows takes 2.5 - 3.5 us on the GPU, less than its launch costs the host.
 #include "actq8.h"
 #include "../../include/s4f.h"
 #include <algorithm>
